@@ -24,13 +24,15 @@
  *   - thread-safe and re-entrant: no mutable global state except the debug and
  *     profiling switches below, which are meant for tests and benchmarks;
  *   - dtype codes: PA_F32 = 0, PA_BF16 = 1, PA_FP8_E4M3FN = 2 (OCP e4m3fn,
- *     KV cache only, with one float scale per (block, kv head)).
+ *     KV cache only, with one float scale per (block, kv head)), PA_INT8 = 4 (signed codes,
+ *     KV cache only, with one float scale per (token, kv head)).
  *
  * Tensor layouts (row-major, contiguous)
  *   q, out (decode)      [B, Hq, D]
  *   q, out (prefill)     [B, T, Hq, D]; rows t >= query_lens[b] are padding
  *   k_cache, v_cache     [num_blocks, block_size, Hkv, D]
- *   k_scale, v_scale     [num_blocks, Hkv] float (fp8 KV only, else NULL)
+ *   k_scale, v_scale     [num_blocks, Hkv] float for fp8 KV, [num_blocks, Hkv, block_size] float (16-byte
+ *                        aligned) for int8 KV, else NULL
  *   block_tables         [B, max_blocks_per_seq] int32, logical -> physical block
  *   seq_lens             [B] int32, keys visible to the last query token
  *   query_lens           [B] int32, new tokens of each sequence (<= T, <= seq_lens[b])
@@ -46,7 +48,7 @@
 extern "C" {
 #endif
 
-enum { PA_F32 = 0, PA_BF16 = 1, PA_FP8_E4M3FN = 2 };
+enum { PA_F32 = 0, PA_BF16 = 1, PA_FP8_E4M3FN = 2, PA_INT8 = 4 };
 
 /* Library version: major * 10000 + minor * 100 + patch (a minor step marks a changed or added signature). */
 int pa_version(void);
@@ -118,7 +120,8 @@ size_t pa_decode_workspace_bytes_for(int B, int Hq, int Hkv, int D, int block_si
  * The result does not depend on the split beyond the order of float32 sums.
  * max_seq_len: upper bound of seq_lens (sizes the grid and picks the kernel; 0 =
  * max_blocks_per_seq * block_size).  seq_lens[b] == 0 yields zeros.
- * q_dtype / kv_dtype: (F32, F32), (BF16, BF16) or (BF16, FP8_E4M3FN).
+ * q_dtype / kv_dtype: (F32, F32), (BF16, BF16), (BF16, FP8_E4M3FN) or, on the MFMA kernels' shapes only,
+ *   (BF16, INT8).
  * sinks: NULL, or [Hq] float32 per-head logits that join every softmax as one more column and
  *   are dropped afterwards (examples/models/gpt_oss/kernels/attention.py:137-148): they only
  *   enlarge the denominator.  sliding_window: 0, or W >= 1: the query at position p sees the W
@@ -167,7 +170,7 @@ int pa_decode_noalloc(const void* q, const void* k_cache, const void* v_cache,
  * from HBM once per kv head however many tokens are verified, at decode's bandwidth.
  *   q, out       [B, T, Hq, D] bf16; rows t >= query_lens[b] are padding, zero in out
  *   seq_lens[b]  context length including the query tokens, whose K/V are already in the pool
- *   kv_dtype     PA_BF16 or PA_FP8_E4M3FN (then k_scale / v_scale [num_blocks, Hkv] f32)
+ *   kv_dtype     PA_BF16, PA_FP8_E4M3FN or PA_INT8 (the latter two with k_scale / v_scale)
  *   workspace    pa_verify_workspace_bytes(B, T, Hq, D) bytes, 16-byte aligned
  *   sinks, sliding_window   as for pa_decode (the window counts back from each query token's own position)
  *   max_seq_len  0, or a host-known upper bound of seq_lens (longer contexts are read up to the bound).  The table
@@ -354,6 +357,9 @@ int pa_gather_kv(const void* cache, const int32_t* block_tables, const int32_t* 
  *                 maximum of absmax / 448 over the tokens a block holds; when a write raises it the
  *                 block's earlier rows are re-encoded; a block whose first row is written is fresh.
  *                 The fp8 part has no counterpart in the reference.
+ *                 PA_INT8: [num_blocks, Hkv, block_size] float32; the scale of a row (token, kv head) is absmax / 127
+ *                 of that row (1 for zeros), its codes round(x / scale) to nearest even, and no other row is
+ *                 touched; a row with an infinity or a NaN gets the scale NaN.  D in {32, 64, 128, 256}.
  * Blocks being written must belong to one sequence only (shared prefix blocks are read-only).
  * Sequences with query_lens[b] <= 0 or seq_lens[b] < query_lens[b], and table entries outside
  * the pool, write nothing. */
@@ -362,6 +368,26 @@ int pa_kv_write(const void* k_new, const void* v_new, void* k_cache, void* v_cac
                 const int32_t* block_tables, const int32_t* seq_lens, const int32_t* query_lens,
                 int B, int T, int Hkv, int D, int block_size, int max_blocks_per_seq, int num_blocks,
                 int kv_dtype, void* stream);
+
+/* The same for packed rows: token t < query_lens[b] of sequence b is row cu_seqlens[b] + t of k_new / v_new
+ * [total_tokens, Hkv, D] bf16, whose tokens lie k_stride / v_stride elements apart (multiples of 8, at least Hkv * D:
+ * slices of a wider tensor).  At most cu_seqlens[b + 1] - cu_seqlens[b] rows of a sequence count; boundaries outside
+ * [0, total_tokens] count as its ends.  kv_dtype PA_BF16 or PA_INT8; D in {32, 64, 128, 256}. */
+int pa_kv_write_packed(const void* k_new, const void* v_new, long k_stride, long v_stride, const int32_t* cu_seqlens,
+                       int total_tokens, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                       const int32_t* block_tables, const int32_t* seq_lens, const int32_t* query_lens,
+                       int B, int Hkv, int D, int block_size, int max_blocks_per_seq, int num_blocks,
+                       int kv_dtype, void* stream);
+
+/* Reads a paged cache back as dense bf16 rows: token t < seq_lens[b] of sequence b becomes row cu_seqlens[b] + t of
+ * k_out / v_out [total_tokens, Hkv, D] (np.take of the pool, nkipy/src/nkipy/core/tensor.py:575-640, with codes
+ * multiplied by their scales in float32 and rounded once; bf16 pools bit for bit).  A sequence gets at most
+ * cu_seqlens[b + 1] - cu_seqlens[b] rows; rows on which no token falls are left as they are; table entries outside
+ * the pool read as zeros.  kv_dtype PA_BF16, PA_FP8_E4M3FN or PA_INT8; D a multiple of 8. */
+int pa_read_kv(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+               const int32_t* block_tables, const int32_t* seq_lens, const int32_t* cu_seqlens, void* k_out, void* v_out,
+               int total_tokens, int B, int Hkv, int D, int block_size, int max_blocks_per_seq, int num_blocks,
+               int kv_dtype, void* stream);
 
 /* The reference's pre-attention step fused with the KV write: QK RMSNorm
  * (examples/models/qwen3/kernels/rmsnorm.py:4-21, applied at qwen3/kernels/attention.py:78-80),
@@ -377,7 +403,7 @@ int pa_kv_write(const void* k_new, const void* v_new, void* k_cache, void* v_cac
  *                 table are clamped to its last row
  * Arithmetic as the reference's bf16 tensors give it: the norm in float32 rounded once to bf16,
  * every product and sum of the rotation rounded to bf16.  D in {64, 128, 256};
- * kv_dtype PA_BF16 or PA_FP8_E4M3FN (then scales as in pa_kv_write). */
+ * kv_dtype PA_BF16, PA_FP8_E4M3FN or PA_INT8 (the latter two with scales as in pa_kv_write). */
 int pa_qk_norm_rope_kv_write(const void* xq, const void* xk, const void* xv, void* q_out,
                              const void* q_norm_weight, const void* k_norm_weight, float norm_eps,
                              const void* rope_cos, const void* rope_sin, int rope_max_pos,

@@ -18,6 +18,7 @@ _lock = threading.Lock()
 _lib = None
 
 c_int, c_float, c_void_p, c_size_t = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+c_long = ctypes.c_long
 
 
 
@@ -58,6 +59,8 @@ SIGNATURES = {
     "pa_verify_step": (c_int, [c_void_p] * 11 + [c_size_t] + [c_int] * 9 + [c_float, c_int, c_void_p, c_int, c_void_p, c_void_p]),
     "pa_gather_kv": (c_int, [c_void_p] * 4 + [c_int] * 8 + [c_void_p]),
     "pa_kv_write": (c_int, [c_void_p] * 9 + [c_int] * 8 + [c_void_p]),
+    "pa_kv_write_packed": (c_int, [c_void_p] * 2 + [c_long] * 2 + [c_void_p, c_int] + [c_void_p] * 7 + [c_int] * 7 + [c_void_p]),
+    "pa_read_kv": (c_int, [c_void_p] * 9 + [c_int] * 8 + [c_void_p]),
     "pa_qk_norm_rope_kv_write": (c_int, [c_void_p] * 6 + [c_float] + [c_void_p] * 2 + [c_int] + [c_void_p] * 7 + [c_int] * 9 + [c_void_p]),
     "pa_debug_set": (c_int, [c_int, c_int]),
     "pa_profile_enable": (c_int, [c_int]),

@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libpaged_attn.so")
 
-SOURCES = ["pa_capi.hip", "pa_decode_generic.hip", "pa_decode_mfma.hip", "pa_prefill.hip", "pa_prefill_async.hip", "pa_kv_write.hip", "pa_o_proj.hip"]
+SOURCES = ["pa_capi.hip", "pa_decode_generic.hip", "pa_decode_mfma.hip", "pa_prefill.hip", "pa_prefill_async.hip", "pa_kv_write.hip", "pa_kv_read.hip", "pa_o_proj.hip"]
 BENCH_SOURCES = ["pa_probe.hip"]
 BENCH_LIB_PATH = os.path.join(LIB_DIR, "libpa_bench.so")
 
@@ -42,7 +42,7 @@ def _compile(src: str, extra) -> str:
     return obj
 
 
-def build(extra_flags=(), jobs: int = 4) -> str:
+def build(extra_flags=(), jobs: int = 8) -> str:
     """Compile every HIP source and link the shared library; returns its path."""
     os.makedirs(LIB_DIR, exist_ok=True)
     with ThreadPoolExecutor(max_workers=jobs) as ex:

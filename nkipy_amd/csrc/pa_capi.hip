@@ -42,6 +42,8 @@ static std::atomic<int> g_decode_waves{0};
 static std::atomic<int> g_head_major{1};
 static std::atomic<int> g_prefill_impl{0};
 static std::atomic<int> g_lockstep{1};
+// pools of one byte per element
+static bool byte_pool(int kv_dtype) { return kv_dtype == PA_FP8_E4M3FN || kv_dtype == PA_INT8; }
 // The per-tile barrier that keeps the kv-head waves of a balanced decode workgroup on the same tile: debug switch 4,
 // 1 = automatic (the default), 0 = never, 2 = always.  Automatic: on for bf16 pools (the heads' rows of a token are one
 // contiguous piece of DRAM; config 2 80.4 % of HBM peak with it, 77.5 % without), off for fp8 pools (the waves' expansion
@@ -49,7 +51,7 @@ static std::atomic<int> g_lockstep{1};
 static int lockstep_for(int kv_dtype, int bal_ns) {
   const int mode = g_lockstep.load();
   if (bal_ns != 1 || mode == 0) return 0;
-  return mode == 2 || kv_dtype != PA_FP8_E4M3FN ? 1 : 0;
+  return mode == 2 || !byte_pool(kv_dtype) ? 1 : 0;
 }
 static std::atomic<int> g_verify_rows{0};
 static std::atomic<int> g_prefill_split{1};
@@ -230,6 +232,14 @@ static int take_q_transform(const char* who, const pa_q_transform* qt, bool kern
   return 0;
 }
 
+// int8 pools: both scale tables, read 16 bytes at a time
+static int check_int8_scales(const char* who, int kv_dtype, const float* k_scale, const float* v_scale) {
+  if (kv_dtype != PA_INT8) return 0;
+  if (!k_scale || !v_scale) return fail_arg("%s: int8 KV needs k_scale and v_scale", who);
+  if (!aligned16(k_scale) || !aligned16(v_scale)) return fail_arg("%s: the scales of an int8 pool must be 16-byte aligned", who);
+  return 0;
+}
+
 static int num_partitions_for(int max_seq_len, int partition_size) {
   if (max_seq_len <= 0) return 1;
   return (max_seq_len + partition_size - 1) / partition_size;
@@ -277,14 +287,14 @@ static int span_bound(const DecodeParams& p) {
 // 19.2, B = 32 behind 2 K 37.2 / 29.1.  Doubling everything cost where the tokens' count was fine: head dim 64, B = 8
 // behind 1 K 9.7 -> 10.6.)
 static int token_scale(const DecodeParams& p, int kv_dtype) {
-  return g_d64_wide.load() && (p.D <= 64 || kv_dtype == PA_FP8_E4M3FN) ? 2 : 1;
+  return g_d64_wide.load() && (p.D <= 64 || byte_pool(kv_dtype)) ? 2 : 1;
 }
 constexpr int kDecodeSmallCallPartitions = 8;
 static int base_partition(const DecodeParams& p, int kv_dtype) {
   if (num_partitions_for(span_bound(p), p.partition_size) <= kDecodeSmallCallPartitions) return p.partition_size;
   // (not for fp8 pools of head dim 64, which are better off on the balanced kernel there: B = 2 behind 8 K 15.4
   // against 16.6 us, B = 4 behind 6 K 15.6 against 16.4)
-  if (p.D <= 64 && kv_dtype == PA_FP8_E4M3FN) return p.partition_size;
+  if (p.D <= 64 && byte_pool(kv_dtype)) return p.partition_size;
   return p.partition_size * token_scale(p, kv_dtype);
 }
 constexpr long kDecodeSmallCallBytes = 160L << 20;
@@ -297,7 +307,7 @@ constexpr long kDecodeSmallCallPairs = 256;     // (80 while every call took par
 constexpr long kDecodeSmallCallPairsD64 = 320;
 constexpr long kDecodeSmallCallPairsOnePartition = 1024;
 static bool decode_small_call(const DecodeParams& p, int kv_dtype, int max_parts = kDecodeSmallCallPartitions) {
-  const long esz = kv_dtype == PA_FP8_E4M3FN ? 1 : (kv_dtype == PA_BF16 ? 2 : 4);
+  const long esz = byte_pool(kv_dtype) ? 1 : (kv_dtype == PA_BF16 ? 2 : 4);
   if (p.max_seq_len <= 0 || p.partition_size <= 0 || p.partition_size % 32) return false;
   if (num_partitions_for(span_bound(p), base_partition(p, kv_dtype)) > max_parts) return false;
   long pairs_max = p.D <= 64 ? kDecodeSmallCallPairsD64 : kDecodeSmallCallPairs;
@@ -414,13 +424,14 @@ static int plan_decode(const char* who, DecodePlan& pl, const void* q, const voi
                     block_size, max_blocks_per_seq, num_blocks);
   if (partition_size <= 0) return fail_arg("%s: partition_size=%d must be positive", who, partition_size);
   if (!(q_dtype == PA_F32 && kv_dtype == PA_F32) && !(q_dtype == PA_BF16 && kv_dtype == PA_BF16) &&
-      !(q_dtype == PA_BF16 && kv_dtype == PA_FP8_E4M3FN))
+      !(q_dtype == PA_BF16 && byte_pool(kv_dtype)))
     return fail_arg("%s: unsupported dtype pair q=%d kv=%d", who, q_dtype, kv_dtype);
   if (D != 32 && D != 64 && D != 128 && D != 256) return fail_arg("%s: head_dim %d not in {32,64,128,256}", who, D);
   if (B == 0) return 0;
   if (!q || !k_cache || !v_cache || !block_tables || !seq_lens || (out_required && !out))
     return fail_arg("%s: null pointer argument", who);
   if (kv_dtype == PA_FP8_E4M3FN && (!k_scale || !v_scale)) return fail_arg("%s: fp8 KV needs k_scale and v_scale", who);
+  if (int rc = check_int8_scales(who, kv_dtype, k_scale, v_scale)) return rc;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
     return fail_arg("%s: q, k_cache, v_cache and out must be 16-byte aligned", who);
   const long cap = (long)max_blocks_per_seq * block_size;
@@ -446,6 +457,8 @@ static int plan_decode(const char* who, DecodePlan& pl, const void* q, const voi
   // (sinks and a sliding window live in both MFMA kernels; a call forced onto the fixed partitions keeps them)
   const int kind = pl.kind = decode_kind(p, q_dtype, kv_dtype);
   if (kind < 0) return fail_arg("%s: MFMA kernel forced but shape unsupported", who);
+  if (kind == 1 && kv_dtype == PA_INT8)
+    return fail_arg("%s: int8 pools need the matrix-core kernels (head_dim 64 or 128, block_size a power of two >= 16)", who);
   if (kind == 2 && partition_size % 32) return fail_arg("%s: the fixed-partition MFMA kernel needs partition_size %% 32 == 0", who);
   // a small call of short contexts: the whole context as one partition on eight waves, which merge through LDS, so
   // that there is no merge launch.  Per call replayed from a HIP graph (32 / 8 heads of 128, bf16, us, two partitions of
@@ -656,7 +669,7 @@ static int verify_launch(const char* who, const void* q, const void* k_cache, co
     const int n_rows = (Hq / Hkv) * Tc, forced = g_verify_rows.load();
     // (not under a sliding window: the few tiles a launch then sees are better spread over more waves)
     bool wide = n_rows > 16 && (B >= (D == 64 ? 8 : 16) || (n_rows >= 128 && sliding_window == 0)) &&
-                (D == 64 || kv_dtype == PA_FP8_E4M3FN || n_rows > 48);
+                (D == 64 || byte_pool(kv_dtype) || n_rows > 48);
     // fp8 pools at head dim 128: the two-operand wave is the lean form (Q fragments from LDS, V single-buffered; its
     // some fifty spilled registers lie in the start and end of a sequence, not in the tile loop), which the 16-row
     // wave with K and V streamed two tiles deep has overtaken; it only pays on the largest calls (32 / 8 heads,
@@ -670,7 +683,7 @@ static int verify_launch(const char* who, const void* q, const void* k_cache, co
     if (wide) {
       const long bound = max_seq_len > 0 ? std::min<long>(max_seq_len, cap) : cap;
       const long work = (long)B * n_rows * bound;
-      wide = work >= (D == 64 ? 1200000L : kv_dtype == PA_FP8_E4M3FN ? 12L << 20 : 8L << 20);
+      wide = work >= (D == 64 ? 1200000L : byte_pool(kv_dtype) ? 12L << 20 : 8L << 20);
     }
     p.rows_per_wave = forced == 16 || forced == 32 ? forced : (wide ? 32 : 16);
   }
@@ -797,14 +810,15 @@ int pa_verify(const void* q, const void* k_cache, const void* v_cache,
   if (B < 0 || T < 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return fail_arg("pa_verify: bad sizes B=%d T=%d Hq=%d Hkv=%d D=%d", B, T, Hq, Hkv, D);
   if (Hq % Hkv) return fail_arg("pa_verify: Hq=%d is not a multiple of Hkv=%d", Hq, Hkv);
   if (block_size <= 0 || max_blocks_per_seq <= 0 || num_blocks <= 0) return fail_arg("pa_verify: bad paging sizes");
-  if (kv_dtype != PA_BF16 && kv_dtype != PA_FP8_E4M3FN)
-    return fail_arg("pa_verify: kv_dtype must be bf16 or fp8-e4m3fn (got %d)", kv_dtype);
+  if (kv_dtype != PA_BF16 && !byte_pool(kv_dtype))
+    return fail_arg("pa_verify: kv_dtype must be bf16, fp8-e4m3fn or int8 (got %d)", kv_dtype);
   if (T > PA_VERIFY_MAX_TOKENS) return fail_arg("pa_verify: T=%d exceeds %d query tokens per sequence; use pa_prefill", T, PA_VERIFY_MAX_TOKENS);
   if (B == 0 || T == 0) return 0;
   if (B > 65535) return fail_arg("pa_verify: B=%d exceeds 65535", B);
   if (!q || !k_cache || !v_cache || !block_tables || !seq_lens || !query_lens || !out)
     return fail_arg("pa_verify: null pointer argument");
   if (kv_dtype == PA_FP8_E4M3FN && (!k_scale || !v_scale)) return fail_arg("pa_verify: fp8 KV needs k_scale and v_scale");
+  if (int rc = check_int8_scales("pa_verify", kv_dtype, k_scale, v_scale)) return rc;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || !aligned16(workspace))
     return fail_arg("pa_verify: q, k_cache, v_cache, out and workspace must be 16-byte aligned");
   return verify_launch("pa_verify", q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, query_lens, out,
@@ -854,6 +868,9 @@ int pa_prefill(const void* q, const void* k_cache, const void* v_cache,
   if (sliding_window < 0) return fail_arg("pa_prefill: sliding_window=%d must be >= 0 (0 = none)", sliding_window);
   if (Hq % Hkv) return fail_arg("pa_prefill: Hq=%d is not a multiple of Hkv=%d", Hq, Hkv);
   if (dtype != PA_BF16) return fail_arg("pa_prefill: only bf16 queries are supported (dtype=%d)", dtype);
+  if (kv_dtype == PA_INT8)
+    return fail_arg("pa_prefill: int8 pools are read back as bf16 rows (pa_read_kv) for pa_packed_prefill; runs of a few "
+                    "tokens go to pa_verify");
   if (kv_dtype != PA_BF16 && kv_dtype != PA_FP8_E4M3FN)
     return fail_arg("pa_prefill: kv_dtype must be bf16 or fp8-e4m3fn (got %d)", kv_dtype);
   const bool fp8 = kv_dtype == PA_FP8_E4M3FN;
@@ -961,17 +978,20 @@ int pa_kv_write(const void* k_new, const void* v_new, void* k_cache, void* v_cac
   tl_error[0] = 0;
   if (B < 0 || T < 0 || Hkv <= 0 || D <= 0) return fail_arg("pa_kv_write: bad sizes");
   if (block_size <= 0 || max_blocks_per_seq <= 0 || num_blocks <= 0) return fail_arg("pa_kv_write: bad paging sizes");
-  if (kv_dtype != PA_F32 && kv_dtype != PA_BF16 && kv_dtype != PA_FP8_E4M3FN)
+  if (kv_dtype != PA_F32 && kv_dtype != PA_BF16 && !byte_pool(kv_dtype))
     return fail_arg("pa_kv_write: unknown kv_dtype %d", kv_dtype);
   const int src_esz = kv_dtype == PA_F32 ? 4 : 2;
   if ((D * src_esz) % 16 != 0 || (kv_dtype == PA_FP8_E4M3FN && D % 8 != 0))
     return fail_arg("pa_kv_write: D=%d rows must be a multiple of 16 bytes", D);
+  if (kv_dtype == PA_INT8 && !kv_write_rows_supported(D))
+    return fail_arg("pa_kv_write: int8 pools need head_dim 32, 64, 128 or 256 (got %d)", D);
   if ((long)max_blocks_per_seq * block_size > 0x7fffffffL) return fail_arg("pa_kv_write: table capacity exceeds 2^31 tokens");
   if (B == 0 || T == 0) return 0;
   if (B > 65535 || Hkv > 65535) return fail_arg("pa_kv_write: B and Hkv are limited to 65535 (grid dimensions)");
   if (!k_new || !v_new || !k_cache || !v_cache || !block_tables || !seq_lens || !query_lens)
     return fail_arg("pa_kv_write: null pointer argument");
   if (kv_dtype == PA_FP8_E4M3FN && (!k_scale || !v_scale)) return fail_arg("pa_kv_write: fp8 pools need k_scale and v_scale");
+  if (int rc = check_int8_scales("pa_kv_write", kv_dtype, k_scale, v_scale)) return rc;
   if (!aligned16(k_new) || !aligned16(v_new) || !aligned16(k_cache) || !aligned16(v_cache))
     return fail_arg("pa_kv_write: k_new, v_new, k_cache and v_cache must be 16-byte aligned");
   KvWriteParams p;
@@ -981,11 +1001,83 @@ int pa_kv_write(const void* k_new, const void* v_new, void* k_cache, void* v_cac
   p.block_tables = block_tables; p.seq_lens = seq_lens; p.query_lens = query_lens;
   p.B = B; p.T = T; p.Hkv = Hkv; p.D = D; p.block_size = block_size; p.max_blocks = max_blocks_per_seq;
   p.num_blocks = num_blocks; p.kv_dtype = kv_dtype;
+  p.k_stride = p.v_stride = (long)Hkv * D;
   hipStream_t s = (hipStream_t)stream;
   profile_begin(s);
   hipError_t e = launch_kv_write(p, s);
   profile_end(s);
   return check_hip(e, "pa_kv_write launch");
+}
+
+int pa_kv_write_packed(const void* k_new, const void* v_new, long k_stride, long v_stride, const int32_t* cu_seqlens,
+                       int total_tokens, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                       const int32_t* block_tables, const int32_t* seq_lens, const int32_t* query_lens,
+                       int B, int Hkv, int D, int block_size, int max_blocks_per_seq, int num_blocks,
+                       int kv_dtype, void* stream) {
+  tl_error[0] = 0;
+  const char* who = "pa_kv_write_packed";
+  if (B < 0 || total_tokens < 0 || Hkv <= 0 || D <= 0) return fail_arg("%s: bad sizes", who);
+  if (block_size <= 0 || max_blocks_per_seq <= 0 || num_blocks <= 0) return fail_arg("%s: bad paging sizes", who);
+  if (kv_dtype != PA_BF16 && kv_dtype != PA_INT8)
+    return fail_arg("%s: kv_dtype must be bf16 or int8 (got %d): an fp8 pool's scales belong to blocks, whose rows have to be "
+                    "written together (pa_kv_write)", who, kv_dtype);
+  if (!kv_write_rows_supported(D)) return fail_arg("%s: head_dim %d must be 32, 64, 128 or 256", who, D);
+  if ((long)max_blocks_per_seq * block_size > 0x7fffffffL) return fail_arg("%s: table capacity exceeds 2^31 tokens", who);
+  const long row = (long)Hkv * D;
+  if (k_stride < row || v_stride < row || k_stride % 8 || v_stride % 8)
+    return fail_arg("%s: token strides (%ld, %ld elements) must be multiples of 8 and at least Hkv * D = %ld", who, k_stride, v_stride, row);
+  if (B == 0 || total_tokens == 0) return 0;
+  if (Hkv > 65535 || (long)total_tokens + B > 0x7fffffffL) return fail_arg("%s: grid too large (tokens=%d B=%d Hkv=%d)", who, total_tokens, B, Hkv);
+  if (!k_new || !v_new || !cu_seqlens || !k_cache || !v_cache || !block_tables || !seq_lens || !query_lens)
+    return fail_arg("%s: null pointer argument", who);
+  if (int rc = check_int8_scales(who, kv_dtype, k_scale, v_scale)) return rc;
+  if (!aligned16(k_new) || !aligned16(v_new) || !aligned16(k_cache) || !aligned16(v_cache))
+    return fail_arg("%s: k_new, v_new, k_cache and v_cache must be 16-byte aligned", who);
+  KvWriteParams p;
+  memset(&p, 0, sizeof(p));
+  p.k_new = k_new; p.v_new = v_new; p.k_cache = k_cache; p.v_cache = v_cache;
+  p.k_scale = k_scale; p.v_scale = v_scale;
+  p.block_tables = block_tables; p.seq_lens = seq_lens; p.query_lens = query_lens;
+  p.B = B; p.Hkv = Hkv; p.D = D; p.block_size = block_size; p.max_blocks = max_blocks_per_seq;
+  p.num_blocks = num_blocks; p.kv_dtype = kv_dtype;
+  p.cu = cu_seqlens; p.total = total_tokens; p.k_stride = k_stride; p.v_stride = v_stride;
+  hipStream_t s = (hipStream_t)stream;
+  profile_begin(s);
+  hipError_t e = launch_kv_write(p, s);
+  profile_end(s);
+  return check_hip(e, "pa_kv_write_packed launch");
+}
+
+int pa_read_kv(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+               const int32_t* block_tables, const int32_t* seq_lens, const int32_t* cu_seqlens, void* k_out, void* v_out,
+               int total_tokens, int B, int Hkv, int D, int block_size, int max_blocks_per_seq, int num_blocks,
+               int kv_dtype, void* stream) {
+  tl_error[0] = 0;
+  const char* who = "pa_read_kv";
+  if (B < 0 || total_tokens < 0 || Hkv <= 0 || D <= 0) return fail_arg("%s: bad sizes", who);
+  if (block_size <= 0 || max_blocks_per_seq <= 0 || num_blocks <= 0) return fail_arg("%s: bad paging sizes", who);
+  if (kv_dtype != PA_BF16 && !byte_pool(kv_dtype)) return fail_arg("%s: kv_dtype must be bf16, fp8-e4m3fn or int8 (got %d)", who, kv_dtype);
+  if (D % 8) return fail_arg("%s: head_dim %d must be a multiple of 8", who, D);
+  if ((long)max_blocks_per_seq * block_size > 0x7fffffffL) return fail_arg("%s: table capacity exceeds 2^31 tokens", who);
+  if ((long)Hkv * D > 0x3ffffffL) return fail_arg("%s: rows of %ld elements are too long", who, (long)Hkv * D);
+  if (B == 0 || total_tokens == 0) return 0;
+  if ((long)total_tokens + B > 0x7fffffffL) return fail_arg("%s: grid too large (tokens=%d B=%d)", who, total_tokens, B);
+  if (!k_cache || !v_cache || !block_tables || !seq_lens || !cu_seqlens || !k_out || !v_out)
+    return fail_arg("%s: null pointer argument", who);
+  if (byte_pool(kv_dtype) && (!k_scale || !v_scale)) return fail_arg("%s: pools of codes need k_scale and v_scale", who);
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_out) || !aligned16(v_out))
+    return fail_arg("%s: k_cache, v_cache, k_out and v_out must be 16-byte aligned", who);
+  KvReadParams p;
+  memset(&p, 0, sizeof(p));
+  p.k_cache = k_cache; p.v_cache = v_cache; p.k_scale = k_scale; p.v_scale = v_scale;
+  p.block_tables = block_tables; p.seq_lens = seq_lens; p.cu = cu_seqlens; p.k_out = k_out; p.v_out = v_out;
+  p.B = B; p.Hkv = Hkv; p.D = D; p.block_size = block_size; p.block_shift = ilog2_exact(block_size);
+  p.max_blocks = max_blocks_per_seq; p.num_blocks = num_blocks; p.total = total_tokens; p.kv_dtype = kv_dtype;
+  hipStream_t s = (hipStream_t)stream;
+  profile_begin(s);
+  hipError_t e = launch_kv_read(p, s);
+  profile_end(s);
+  return check_hip(e, "pa_read_kv launch");
 }
 
 int pa_qk_norm_rope_kv_write(const void* xq, const void* xk, const void* xv, void* q_out,
@@ -999,8 +1091,8 @@ int pa_qk_norm_rope_kv_write(const void* xq, const void* xk, const void* xv, voi
   if (B < 0 || T < 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return fail_arg("pa_qk_norm_rope_kv_write: bad sizes");
   if (block_size <= 0 || max_blocks_per_seq <= 0 || num_blocks <= 0 || rope_max_pos <= 0)
     return fail_arg("pa_qk_norm_rope_kv_write: bad paging or table sizes");
-  if (kv_dtype != PA_BF16 && kv_dtype != PA_FP8_E4M3FN)
-    return fail_arg("pa_qk_norm_rope_kv_write: kv_dtype must be bf16 or fp8-e4m3fn (got %d)", kv_dtype);
+  if (kv_dtype != PA_BF16 && !byte_pool(kv_dtype))
+    return fail_arg("pa_qk_norm_rope_kv_write: kv_dtype must be bf16, fp8-e4m3fn or int8 (got %d)", kv_dtype);
   if (!kv_write_xform_supported(D)) return fail_arg("pa_qk_norm_rope_kv_write: head_dim %d must be 64, 128 or 256", D);
   if ((long)max_blocks_per_seq * block_size > 0x7fffffffL) return fail_arg("pa_qk_norm_rope_kv_write: table capacity exceeds 2^31 tokens");
   if (B == 0 || T == 0) return 0;
@@ -1010,6 +1102,7 @@ int pa_qk_norm_rope_kv_write(const void* xq, const void* xk, const void* xv, voi
   if ((xq == nullptr) != (q_out == nullptr))
     return fail_arg("pa_qk_norm_rope_kv_write: xq and q_out must both be given, or both be NULL (K and V only)");
   if (kv_dtype == PA_FP8_E4M3FN && (!k_scale || !v_scale)) return fail_arg("pa_qk_norm_rope_kv_write: fp8 pools need k_scale and v_scale");
+  if (int rc = check_int8_scales("pa_qk_norm_rope_kv_write", kv_dtype, k_scale, v_scale)) return rc;
   if (!aligned16(xq) || !aligned16(xk) || !aligned16(xv) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache))
     return fail_arg("pa_qk_norm_rope_kv_write: xq, xk, xv, q_out, k_cache and v_cache must be 16-byte aligned");
   if (!aligned16(rope_cos) || !aligned16(rope_sin) || !aligned16(q_norm_weight) || !aligned16(k_norm_weight))
@@ -1025,6 +1118,7 @@ int pa_qk_norm_rope_kv_write(const void* xq, const void* xk, const void* xv, voi
   p.q_norm_weight = (const uint16_t*)q_norm_weight; p.k_norm_weight = (const uint16_t*)k_norm_weight;
   p.rope_cos = (const uint16_t*)rope_cos; p.rope_sin = (const uint16_t*)rope_sin;
   p.norm_eps = norm_eps; p.rope_max_pos = rope_max_pos;
+  p.k_stride = p.v_stride = (long)Hkv * D;
   hipStream_t s = (hipStream_t)stream;
   profile_begin(s);
   hipError_t e = launch_kv_write(p, s);
@@ -1237,7 +1331,7 @@ int pa_verify_step(const void* q, const pa_new_kv* new_kv, void* k_cache, void* 
   }
   if (B == 0 || T == 0) return 0;
   if (Hq % Hkv) return fail_arg("%s: Hq=%d is not a multiple of Hkv=%d", who, Hq, Hkv);
-  if (kv_dtype != PA_BF16 && kv_dtype != PA_FP8_E4M3FN) return fail_arg("%s: kv_dtype must be bf16 or fp8-e4m3fn", who);
+  if (kv_dtype != PA_BF16 && !byte_pool(kv_dtype)) return fail_arg("%s: kv_dtype must be bf16, fp8-e4m3fn or int8", who);
   if (!q) return fail_arg("%s: null pointer argument", who);
   const long M = (long)B * T;
   hipStream_t s = (hipStream_t)stream;

@@ -91,6 +91,24 @@ template <> struct Store<uint16_t> {
   }
 };
 
+// ---- packed rows -------------------------------------------------------------------
+// Sequence i of n owns rows [cu[i], cu[i + 1]) of a packed tensor of `total` rows.  Work is dealt in tiles of 2^shift rows
+// of one sequence; tile t of sequence i has the number floor(cu[i] / 2^shift) + i + t, which no other tile has and
+// which needs no pass over the lengths: from one sequence to the next it grows by floor(cu[i + 1] / 2^shift) -
+// floor(cu[i] / 2^shift) + 1 >= ceil(len / 2^shift).  So floor(total / 2^shift) + n numbers cover every tile (some have
+// none), and the sequence of a number is found by bisection.  Boundaries outside [0, total] count as its ends.
+__device__ __forceinline__ int packed_row(const int32_t* cu, int i, int total) { return min(max(cu[i], 0), total); }
+__device__ __forceinline__ int packed_find(const int32_t* cu, int n, int total, int shift, int slot, int* tile) {
+  int lo = 0, hi = n;                     // the last i with first_slot(i) <= slot lies in [lo, hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((packed_row(cu, mid, total) >> shift) + mid <= slot) lo = mid;
+    else hi = mid;
+  }
+  *tile = slot - ((packed_row(cu, lo, total) >> shift) + lo);
+  return lo;
+}
+
 // ---- Q transform on load ---------------------------------------------------------
 // The reference's pre-attention step on Q (QK RMSNorm, examples/models/qwen3/kernels/rmsnorm.py:4-21;
 // RoPE at the token's absolute position, rope.py:23-48) applied by the attention kernel to the Q
@@ -203,7 +221,7 @@ struct DecodeParams {
   const void* q;            // [B, Hq, D]; [B, T, Hq, D] for a multi-token call
   const void* k_cache;      // [num_blocks, block_size, Hkv, D]
   const void* v_cache;
-  const float* k_scale;     // [num_blocks, Hkv] or null
+  const float* k_scale;     // fp8 [num_blocks, Hkv], int8 [num_blocks, Hkv, block_size], else null
   const float* v_scale;
   const int32_t* block_tables;  // [B, max_blocks]
   const int32_t* seq_lens;      // [B]
@@ -287,16 +305,22 @@ bool prefill_async_supported(const PrefillParams& p);
 // ---- gather ------------------------------------------------------------------------
 // ---- paged KV write --------------------------------------------------------------
 struct KvWriteParams {
-  const void* k_new;        // [B, T, Hkv, D] bf16 (fp32 for an fp32 pool)
+  const void* k_new;        // [B, T, Hkv, D] bf16 (fp32 for an fp32 pool); packed form [total, Hkv, D]
   const void* v_new;
   void* k_cache;            // [num_blocks, block_size, Hkv, D]
   void* v_cache;
-  float* k_scale;           // [num_blocks, Hkv] (fp8 pools) or null
+  float* k_scale;           // fp8 [num_blocks, Hkv], int8 [num_blocks, Hkv, block_size], else null
   float* v_scale;
   const int32_t* block_tables;
   const int32_t* seq_lens;
   const int32_t* query_lens;
   int B, T, Hkv, D, block_size, max_blocks, num_blocks, kv_dtype;
+  // packed form (int8 and bf16 pools): sequence b's new rows are rows cu[b] .. of k_new / v_new, whose consecutive tokens
+  // lie k_stride / v_stride elements apart; null for the padded form
+  const int32_t* cu;        // [B + 1]
+  int total;                // rows of k_new / v_new
+  long k_stride, v_stride;
+  int tok_shift;            // row-wise kernel: log2 of the tokens a workgroup covers
   // pre-attention transform (all null / zero for a plain write): RMSNorm weights [D] bf16 (null: no
   // norm), RoPE tables [rope_max_pos, D/2] bf16, Q rows [B, T, Hq, D] bf16 transformed into q_out
   const void* q_in;
@@ -309,7 +333,23 @@ struct KvWriteParams {
   int Hq, rope_max_pos;
 };
 hipError_t launch_kv_write(const KvWriteParams& p, hipStream_t s);
+bool kv_write_rows_supported(int D);    // head dims of the row-wise kernel (int8 pools, packed rows)
 bool kv_write_xform_supported(int D);   // head dims the fused RMSNorm + RoPE write is built for
+
+// ---- reading a paged cache back as dense bf16 rows ------------------------------------------
+struct KvReadParams {
+  const void* k_cache;      // [num_blocks, block_size, Hkv, D]
+  const void* v_cache;
+  const float* k_scale;     // fp8 [num_blocks, Hkv], int8 [num_blocks, Hkv, block_size], else null
+  const float* v_scale;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  const int32_t* cu;        // [B + 1]: token t of sequence b is row cu[b] + t of the outputs
+  void* k_out;              // [total, Hkv, D] bf16
+  void* v_out;
+  int B, Hkv, D, block_size, block_shift, max_blocks, num_blocks, total, kv_dtype;
+};
+hipError_t launch_kv_read(const KvReadParams& p, hipStream_t s);
 
 // ---- post-attention output projection ---------------------------------------------------
 struct OProjParams {

@@ -35,12 +35,26 @@
 // applied to the fp32 scores (K) and folded into P (V), so the dequantised
 // cache is never written anywhere.
 //
+// int8 KV: the same with a float32 scale per (token, kv head) and codes that a conversion to float32 and a
+// packing of high halves turn into bf16 (every code is a bf16 value).
+//
 // Math restated: attention.py:112-144 + softmax.py:4-6 in one pass; the merge
 // of partitions is  m = max m_i, l = sum l_i 2^(m_i-m), o = sum o_i l_i 2^(m_i-m)/l.
+#include <type_traits>
+
 #include "pa_common.h"
 
 namespace pa {
 namespace {
+
+// What the pool holds: bf16, OCP e4m3fn codes with a scale per (block, kv head), int8 codes with one per (token, kv head)
+constexpr int KV_BF16 = 0, KV_FP8 = 1, KV_I8 = 2;
+
+// signed byte BYTE of w as a float (one instruction: the conversion reads the byte through its operand selector)
+template <int BYTE>
+__device__ __forceinline__ float i8_to_float(uint32_t w) {
+  return (float)(int)(int8_t)(w >> (8 * BYTE));
+}
 
 // N dwords per lane; NT: a streaming (non-temporal) load, for bytes that are read once
 template <int N, bool NT = false> struct VecLoad;
@@ -81,18 +95,18 @@ __device__ __forceinline__ bf16x8_t as_bf16x8(uint32_t a, uint32_t b, uint32_t c
 // One 32-token tile as loaded (raw bits), K and V halves separately so that
 // their register lifetimes can interleave (K of tile n dies after the scores,
 // which frees its registers for V of tile n+1).
-template <int D, bool FP8>
+template <int D, int KV>
 struct KTile {
-  static constexpr int KLD = FP8 ? D / 64 : D / 32;        // 16-byte K loads per 16-token sub-tile
+  static constexpr int KLD = KV != KV_BF16 ? D / 64 : D / 32;        // 16-byte K loads per 16-token sub-tile
   uint32_t k[2][KLD][4];
-  float ksc[2];             // fp8 only: scales of the two 16-token halves
+  float ksc[KV == KV_I8 ? 8 : 2];      // fp8: scales of the two 16-token halves; int8: of the lane's eight tokens
 };
-template <int D, bool FP8>
+template <int D, int KV>
 struct VTile {
-  static constexpr int VEC = D / 16;                       // d's per lane for V
-  static constexpr int VW = (VEC * (FP8 ? 1 : 2)) / 4;     // dwords per V load
+  static constexpr int VEC = D / 16;                                 // d's per lane for V
+  static constexpr int VW = (VEC * (KV != KV_BF16 ? 1 : 2)) / 4;     // dwords per V load
   uint32_t v[8][VW];
-  float vsc[2];
+  float vsc[KV == KV_I8 ? 8 : 2];
 };
 
 // Per-wavefront streaming state: Q fragments, online-softmax state and output
@@ -113,13 +127,13 @@ struct VTile {
 // the 16-byte pieces it wrote itself (no conflicts, no barrier), and V is single-
 // buffered: the next tile's V is requested right after the current P.V.
 // Where the 8-element chunks of a Q row sit in the Q^T operand: lane (g, r) holds, in k-step s,
-// chunk 4 s + g (bf16 pools) or 8 (s >> 1) + 2 g + (s & 1) (fp8 pools, whose K loads cover 16
+// chunk 4 s + g (bf16 pools) or 8 (s >> 1) + 2 g + (s & 1) (pools of bytes, whose K loads cover 16
 // elements of a row per lane).  g is lane >> 4.
-template <bool FP8>
+template <bool BYTES>
 struct QOperandLayout {
-  static __device__ __forceinline__ int chunk(int s, int g) { return FP8 ? 8 * (s >> 1) + 2 * g + (s & 1) : 4 * s + g; }
-  static constexpr int slot_xor(int bit) { return FP8 ? (bit == 1 ? 1 : bit == 8 ? 2 : 0) : (bit >> 2); }
-  static constexpr int lane_xor(int bit) { return FP8 ? (bit == 2 ? 16 : bit == 4 ? 32 : 0) : (bit == 1 ? 16 : bit == 2 ? 32 : 0); }
+  static __device__ __forceinline__ int chunk(int s, int g) { return BYTES ? 8 * (s >> 1) + 2 * g + (s & 1) : 4 * s + g; }
+  static constexpr int slot_xor(int bit) { return BYTES ? (bit == 1 ? 1 : bit == 8 ? 2 : 0) : (bit >> 2); }
+  static constexpr int lane_xor(int bit) { return BYTES ? (bit == 2 ? 16 : bit == 4 ? 32 : 0) : (bit == 1 ? 16 : bit == 2 ? 32 : 0); }
 };
 
 // NEWROW (decode, bf16 pools, fixed partitions): the sequence's newest token is not in the pool yet but comes with
@@ -127,17 +141,18 @@ struct QOperandLayout {
 // registers and puts them in the place of what the tile loads brought for that token (and for the rows behind it,
 // which the loads redirect to it), so the scores and the output are those of a pool that already held the row; the
 // same wave stores the row in the pool for the steps to come.
-template <int D, bool FP8, bool MULTI = false, int R = 1, bool LEAN = false, bool SV = false, bool NEWROW = false>
+template <int D, int KV, bool MULTI = false, int R = 1, bool LEAN = false, bool SV = false, bool NEWROW = false>
 struct DecodeWave {
-  static_assert(!NEWROW || (!FP8 && R == 1 && !LEAN && !SV), "the new-row forms are bf16, one 16-row operand per wave");
-  using KT = KTile<D, FP8>;
-  using VT = VTile<D, FP8>;
+  static constexpr bool FP8 = KV == KV_FP8, I8 = KV == KV_I8, BYTES = KV != KV_BF16;
+  static_assert(!NEWROW || (!BYTES && R == 1 && !LEAN && !SV), "the new-row forms are bf16, one 16-row operand per wave");
+  using KT = KTile<D, KV>;
+  using VT = VTile<D, KV>;
   static constexpr int VEC = VT::VEC, KLD = KT::KLD, VW = VT::VW;
   static constexpr int KSTEPS = D / 32;
-  static constexpr int ESZ = FP8 ? 1 : 2;
+  static constexpr int ESZ = BYTES ? 1 : 2;
   // K streamed too (with V), for bf16 pools: config 2 kernel 169.3 -> 166.4 us, verify 180.0 -> 178.0; on the fp8
   // pool, whose expansion already costs vector instructions, the rearrangement costs more than it brings (375.5 -> 379.5)
-  static constexpr bool SK = SV && !FP8 && D * ESZ >= 128;
+  static constexpr bool SK = SV && !BYTES && D * ESZ >= 128;
 
   const DecodeParams& p;
   int hk, hbase, nheads;     // kv head, first (virtual) q head, valid rows of this wave
@@ -182,7 +197,7 @@ struct DecodeWave {
     nheads = min(16 * R, n_rows - jbase);
     r = lane & 15;
     g = lane >> 4;
-    krow = 4 * (r & 3) + (r >> 2);
+    krow = I8 ? r : 4 * (r & 3) + (r >> 2);
     k_first_half = krow < 8;
     kperm_addr[0] = 4 * (8 * (krow & 7) + g);
     kperm_addr[1] = 4 * (8 * (krow & 7) + 4 + g);
@@ -314,13 +329,13 @@ struct DecodeWave {
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
         // d range of k-slots 8g..8g+7 in step s (must mirror the K loads below)
-        const int d0 = FP8 ? ((4 * (s >> 1) + g) * 16 + (s & 1) * 8) : ((4 * s + g) * 8);
+        const int d0 = BYTES ? ((4 * (s >> 1) + g) * 16 + (s & 1) * 8) : ((4 * s + g) * 8);
         q.qraw[rg][s] = make_uint4(0, 0, 0, 0);
         if (row_valid) q.qraw[rg][s] = *(const uint4*)(qrow + d0);
       }
       if (p.qt.cos) {
         const int qpos = MULTI ? row_end[rg] - 1 : last;
-        norm_rope_fetch<D / 8, KSTEPS, QOperandLayout<FP8>>(p.qt, min(max(qpos, 0), p.qt.max_pos - 1), g, q.qc[rg]);
+        norm_rope_fetch<D / 8, KSTEPS, QOperandLayout<BYTES>>(p.qt, min(max(qpos, 0), p.qt.max_pos - 1), g, q.qc[rg]);
       }
     }
   }
@@ -341,7 +356,7 @@ struct DecodeWave {
             x[s][2 * j + 1] = bf16_bits_to_float(w[j] >> 16);
           }
         }
-        norm_rope_apply<D / 8, KSTEPS, QOperandLayout<FP8>>(x, p.qt, g, q.qc[rg]);
+        norm_rope_apply<D / 8, KSTEPS, QOperandLayout<BYTES>>(x, p.qt, g, q.qc[rg]);
 #pragma unroll
         for (int s = 0; s < KSTEPS; ++s) {
           qraw[s].x = pack_bf16x2(x[s][0], x[s][1]); qraw[s].y = pack_bf16x2(x[s][2], x[s][3]);
@@ -426,6 +441,20 @@ struct DecodeWave {
     return tr;
   }
 
+  // Token of the tile that slot j of this lane's eight score / probability / V-row slots stands for.  int8 pools keep
+  // the matrix instruction's own order, four consecutive tokens per lane and half, so that a lane's scales are two
+  // 16-byte loads (a scale per token, contiguous in the pool) instead of eight of 4 bytes.
+  __device__ __forceinline__ int slot_token(int j) const { return I8 ? 16 * (j >> 2) + 4 * g + (j & 3) : 4 * j + g; }
+  // int8: scales [num_blocks, Hkv, block_size] of the lane's tokens of the tile at t0.  Those of tokens past the context
+  // are whatever the pool holds there; what they multiply is masked by selection.
+  __device__ __forceinline__ void load_token_scales(const float* tbl, float* sc, const TileRows& tr, int t0) const {
+    const int bmask = p.block_size - 1;
+    const float4 a = *(const float4*)(tbl + ((long)tr.blk0 * p.Hkv + hk) * p.block_size + (t0 & bmask) + 4 * g);
+    const float4 b = *(const float4*)(tbl + ((long)tr.blk1 * p.Hkv + hk) * p.block_size + ((t0 + 16) & bmask) + 4 * g);
+    sc[0] = a.x; sc[1] = a.y; sc[2] = a.z; sc[3] = a.w;
+    sc[4] = b.x; sc[5] = b.y; sc[6] = b.z; sc[7] = b.w;
+  }
+
   // Loads of the tile starting at token t0.  Rows past the context are
   // redirected to the last valid token so that no stale pool bytes (which could
   // be NaN patterns) ever reach the matrix cores.
@@ -435,6 +464,7 @@ struct DecodeWave {
       tl.ksc[0] = p.k_scale[(long)tr.blk0 * p.Hkv + hk];
       tl.ksc[1] = p.k_scale[(long)tr.blk1 * p.Hkv + hk];
     }
+    if (I8) load_token_scales(p.k_scale, tl.ksc, tr, t0);
     if (SK) {
       // One instruction = 8 rows x one whole 128-byte line (lane: row 8 hf + lane / 8 of the sub-tile in tile
       // order, 16-byte chunk lane % 8), so that a streamed line is used up by the instruction that fetches it; slot
@@ -490,9 +520,10 @@ struct DecodeWave {
       tl.vsc[0] = p.v_scale[(long)tr.blk0 * p.Hkv + hk];
       tl.vsc[1] = p.v_scale[(long)tr.blk1 * p.Hkv + hk];
     }
+    if (I8) load_token_scales(p.v_scale, tl.vsc, tr, t0);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int tl_ = min(4 * j + g, tr.lmax);
+      const int tl_ = min(slot_token(j), tr.lmax);
       const long row = (tl_ < 16) ? tr.row0 + tl_ : tr.row1 + (tl_ - 16);
       const char* rowp = vbase + row * row_stride;
       VecLoad<VW, SV>::get(rowp + r * (VEC * ESZ), tl.v[j]);
@@ -513,7 +544,7 @@ struct DecodeWave {
 #pragma unroll
     for (int rg = 0; rg < R; ++rg) sacc[rg][0] = sacc[rg][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     // each Q fragment is fetched once and used for both 16-token halves
-    if (!FP8) {
+    if (!BYTES) {
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
 #pragma unroll
@@ -537,8 +568,13 @@ struct DecodeWave {
           k_chunk(tl, u, s, kc);
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
-            w[u][2 * d] = fp8x2_to_bf16x2<false>(kc[d]);
-            w[u][2 * d + 1] = fp8x2_to_bf16x2<true>(kc[d]);
+            if (I8) {
+              w[u][2 * d] = pack_hi16(i8_to_float<0>(kc[d]), i8_to_float<1>(kc[d]));
+              w[u][2 * d + 1] = pack_hi16(i8_to_float<2>(kc[d]), i8_to_float<3>(kc[d]));
+            } else {
+              w[u][2 * d] = fp8x2_to_bf16x2<false>(kc[d]);
+              w[u][2 * d + 1] = fp8x2_to_bf16x2<true>(kc[d]);
+            }
           }
         }
 #pragma unroll
@@ -562,8 +598,8 @@ struct DecodeWave {
         const float sc = FP8 ? p.scale_log2e * tl.ksc[u] : p.scale_log2e;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int tok = t0 + 16 * u + 4 * i + g;
-          const float x = sacc[rg][u][i] * sc;
+          const int tok = t0 + slot_token(4 * u + i);
+          const float x = sacc[rg][u][i] * (I8 ? p.scale_log2e * tl.ksc[(4 * u + i) % (I8 ? 8 : 2)] : sc);
           sv[4 * u + i] = tok < lim ? x : -INFINITY;
         }
       }
@@ -573,7 +609,7 @@ struct DecodeWave {
         const int lo = (MULTI ? row_end[rg] : last + 1) - p.window;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (t0 + 16 * (i >> 2) + 4 * (i & 3) + g < lo) sv[i] = -INFINITY;
+          if (t0 + slot_token(i) < lo) sv[i] = -INFINITY;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) tmax = fmaxf(tmax, sv[i]);
@@ -597,6 +633,10 @@ struct DecodeWave {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { pr[i] *= vt.vsc[0]; pr[4 + i] *= vt.vsc[1]; }
       }
+      if (I8) {      // (a masked slot's scale may be anything, not a number included)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pr[i] = sv[i] == -INFINITY ? 0.f : pr[i] * vt.vsc[i % (I8 ? 8 : 2)];
+      }
       pf[rg] = as_bf16x8(pack_bf16x2(pr[0], pr[1]), pack_bf16x2(pr[2], pr[3]),
                          pack_bf16x2(pr[4], pr[5]), pack_bf16x2(pr[6], pr[7]));
     }
@@ -604,7 +644,27 @@ struct DecodeWave {
 
   // V^T fragments by in-register transpose, then O^T += V^T P^T.
   __device__ __forceinline__ void accumulate_pv(const VT& tl) {
-    if (!FP8) {
+    if (I8) {
+      // the conversion's result is a float whose high half is the value's bf16 (integers up to 127 are exact): two
+      // tokens' high halves side by side are the operand's word, so the transpose is the packing
+#pragma unroll
+      for (int dw = 0; dw < VW; ++dw) {
+        auto column = [&](auto eb) __attribute__((always_inline)) {
+          uint32_t w[4];
+#pragma unroll
+          for (int jp = 0; jp < 4; ++jp)
+            w[jp] = pack_hi16(i8_to_float<decltype(eb)::value>(tl.v[2 * jp][dw]), i8_to_float<decltype(eb)::value>(tl.v[2 * jp + 1][dw]));
+#pragma unroll
+          for (int rg = 0; rg < R; ++rg)
+            oacc[rg][4 * dw + decltype(eb)::value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                as_bf16x8(w[0], w[1], w[2], w[3]), pf[rg], oacc[rg][4 * dw + decltype(eb)::value], 0, 0, 0);
+        };
+        column(std::integral_constant<int, 0>{});
+        column(std::integral_constant<int, 1>{});
+        column(std::integral_constant<int, 2>{});
+        column(std::integral_constant<int, 3>{});
+      }
+    } else if (!FP8) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
@@ -836,9 +896,9 @@ __host__ __device__ __forceinline__ int head_slots_of(const DecodeParams& p) {
 // bound lies before it), which leaves an empty partial (m = -inf, l = 0); rows past the query length come out as zeros.
 // NEWROW: the step's new K / V row comes with the call (see DecodeWave); the workgroup of the partition that holds
 // token ctx - 1 attends to it from registers and stores it.
-template <int D, bool FP8, int NW, bool MULTI = false, bool NEWROW = false>
+template <int D, int KV, int NW, bool MULTI = false, bool NEWROW = false>
 __global__ __launch_bounds__(NW * 64, NW > 4 ? 1 : 2) void decode_mfma_kernel(DecodeParams p) {
-  using W = DecodeWave<D, FP8, MULTI, 1, false, false, NEWROW>;
+  using W = DecodeWave<D, KV, MULTI, 1, false, false, NEWROW>;
   constexpr int VEC = W::VEC;
   constexpr int OSTRIDE = D + 16;   // LDS row stride (floats) for the merge
 
@@ -1140,10 +1200,10 @@ __device__ __forceinline__ void find_tile(const DecodeParams& p, int lane, int f
   *start_out = start;
 }
 
-template <int D, bool FP8, bool MULTI, int R, bool SV>
+template <int D, int KV, bool MULTI, int R, bool SV>
 __global__ __launch_bounds__(512, 2) void decode_balanced_kernel(DecodeParams p) {
   constexpr bool LEAN = R == 2 && D == 128;
-  using W = DecodeWave<D, FP8, MULTI, R, LEAN, SV>;
+  using W = DecodeWave<D, KV, MULTI, R, LEAN, SV>;
   __shared__ uint4 q_store[LEAN ? 8 * R * W::KSTEPS * 64 : 1];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1313,7 +1373,7 @@ __global__ __launch_bounds__(256) void decode_balanced_reduce_kernel(DecodeParam
   }
 }
 
-template <int D, bool FP8>
+template <int D, int KV>
 hipError_t launch_typed(const DecodeParams& p, int waves, hipStream_t s) {
   const int n_rep = p.Hq / p.Hkv;
   const int slots = head_slots_of(p);                  // Hkv x 16-row groups of a kv head's rows
@@ -1322,42 +1382,42 @@ hipError_t launch_typed(const DecodeParams& p, int waves, hipStream_t s) {
   if (p.query_lens) {      // multi-token rows: the four-wave form
     if (p.rows_per_wave != 16) return hipErrorInvalidValue;
     if (p.new_k) {
-      if constexpr (FP8) return hipErrorInvalidValue;
+      if constexpr (KV != KV_BF16) return hipErrorInvalidValue;
       else {
         if (slots != p.Hkv || p.T > 16 || !p.new_lens) return hipErrorInvalidValue;     // one 16-row wave per kv head holds all its rows
-        hipLaunchKernelGGL((decode_mfma_kernel<D, false, 4, true, true>), grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((decode_mfma_kernel<D, KV_BF16, 4, true, true>), grid, dim3(256), 0, s, p);
         return hipGetLastError();
       }
     }
-    hipLaunchKernelGGL((decode_mfma_kernel<D, FP8, 4, true>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((decode_mfma_kernel<D, KV, 4, true>), grid, dim3(256), 0, s, p);
     return hipGetLastError();
   }
   if (p.new_k) {
-    if constexpr (FP8) {
+    if constexpr (KV != KV_BF16) {
       return hipErrorInvalidValue;
     } else {
       if (waves == 8) {
         if (n_rep > 8) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((decode_mfma_kernel<D, false, 8, false, true>), grid, dim3(512), 0, s, p);
+        hipLaunchKernelGGL((decode_mfma_kernel<D, KV_BF16, 8, false, true>), grid, dim3(512), 0, s, p);
       } else {
-        hipLaunchKernelGGL((decode_mfma_kernel<D, false, 4, false, true>), grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL((decode_mfma_kernel<D, KV_BF16, 4, false, true>), grid, dim3(256), 0, s, p);
       }
       return hipGetLastError();
     }
   }
   switch (waves) {
-    case 1: hipLaunchKernelGGL((decode_mfma_kernel<D, FP8, 1>), grid, dim3(64), 0, s, p); break;
-    case 2: hipLaunchKernelGGL((decode_mfma_kernel<D, FP8, 2>), grid, dim3(128), 0, s, p); break;
+    case 1: hipLaunchKernelGGL((decode_mfma_kernel<D, KV, 1>), grid, dim3(64), 0, s, p); break;
+    case 2: hipLaunchKernelGGL((decode_mfma_kernel<D, KV, 2>), grid, dim3(128), 0, s, p); break;
     case 8:
       if (n_rep > 8) return hipErrorInvalidValue;      // its merge area holds 8 rows per wave
-      hipLaunchKernelGGL((decode_mfma_kernel<D, FP8, 8>), grid, dim3(512), 0, s, p);
+      hipLaunchKernelGGL((decode_mfma_kernel<D, KV, 8>), grid, dim3(512), 0, s, p);
       break;
-    default: hipLaunchKernelGGL((decode_mfma_kernel<D, FP8, 4>), grid, dim3(256), 0, s, p); break;
+    default: hipLaunchKernelGGL((decode_mfma_kernel<D, KV, 4>), grid, dim3(256), 0, s, p); break;
   }
   return hipGetLastError();
 }
 
-template <int D, bool FP8>
+template <int D, int KV>
 hipError_t launch_balanced_typed(const DecodeParams& p, hipStream_t s) {
   const int head_slots = head_slots_of(p);
   dim3 grid(p.bal_gv / p.bal_ns, (head_slots + p.bal_hsw - 1) / p.bal_hsw);
@@ -1365,14 +1425,14 @@ hipError_t launch_balanced_typed(const DecodeParams& p, hipStream_t s) {
   const bool one_reader = head_slots == p.Hkv;         // one wave per kv head: it alone reads that head's V rows
   if (p.B > kScanInRegs) hipLaunchKernelGGL(decode_tile_prefix_kernel, dim3(1), dim3(1024), 0, s, p);
   if (p.query_lens && p.rows_per_wave == 32) {
-    if (one_reader) hipLaunchKernelGGL((decode_balanced_kernel<D, FP8, true, 2, true>), grid, wg, 0, s, p);
-    else hipLaunchKernelGGL((decode_balanced_kernel<D, FP8, true, 2, false>), grid, wg, 0, s, p);
+    if (one_reader) hipLaunchKernelGGL((decode_balanced_kernel<D, KV, true, 2, true>), grid, wg, 0, s, p);
+    else hipLaunchKernelGGL((decode_balanced_kernel<D, KV, true, 2, false>), grid, wg, 0, s, p);
   } else if (p.query_lens) {
-    if (one_reader) hipLaunchKernelGGL((decode_balanced_kernel<D, FP8, true, 1, true>), grid, wg, 0, s, p);
-    else hipLaunchKernelGGL((decode_balanced_kernel<D, FP8, true, 1, false>), grid, wg, 0, s, p);
+    if (one_reader) hipLaunchKernelGGL((decode_balanced_kernel<D, KV, true, 1, true>), grid, wg, 0, s, p);
+    else hipLaunchKernelGGL((decode_balanced_kernel<D, KV, true, 1, false>), grid, wg, 0, s, p);
   } else {
-    if (one_reader) hipLaunchKernelGGL((decode_balanced_kernel<D, FP8, false, 1, true>), grid, wg, 0, s, p);
-    else hipLaunchKernelGGL((decode_balanced_kernel<D, FP8, false, 1, false>), grid, wg, 0, s, p);
+    if (one_reader) hipLaunchKernelGGL((decode_balanced_kernel<D, KV, false, 1, true>), grid, wg, 0, s, p);
+    else hipLaunchKernelGGL((decode_balanced_kernel<D, KV, false, 1, false>), grid, wg, 0, s, p);
   }
   return hipGetLastError();
 }
@@ -1381,7 +1441,7 @@ hipError_t launch_balanced_typed(const DecodeParams& p, hipStream_t s) {
 
 bool decode_mfma_supported(const DecodeParams& p, int q_dtype, int kv_dtype) {
   if (q_dtype != PA_BF16) return false;
-  if (kv_dtype != PA_BF16 && kv_dtype != PA_FP8_E4M3FN) return false;
+  if (kv_dtype != PA_BF16 && kv_dtype != PA_FP8_E4M3FN && kv_dtype != PA_INT8) return false;
   if (p.D != 64 && p.D != 128) return false;
   if (p.block_shift < 4) return false;   // power-of-two block size >= 16
   return true;
@@ -1395,10 +1455,13 @@ bool decode_new_row_supported(const DecodeParams& p, int q_dtype, int kv_dtype) 
 }
 
 hipError_t launch_decode_mfma(const DecodeParams& p, int kv_dtype, int waves, hipStream_t s) {
-  const bool fp8 = kv_dtype == PA_FP8_E4M3FN;
-  if (p.D == 128) return fp8 ? launch_typed<128, true>(p, waves, s) : launch_typed<128, false>(p, waves, s);
-  if (p.D == 64) return fp8 ? launch_typed<64, true>(p, waves, s) : launch_typed<64, false>(p, waves, s);
-  return hipErrorInvalidValue;
+  if (p.D != 64 && p.D != 128) return hipErrorInvalidValue;
+  switch (kv_dtype) {
+    case PA_BF16: return p.D == 128 ? launch_typed<128, KV_BF16>(p, waves, s) : launch_typed<64, KV_BF16>(p, waves, s);
+    case PA_FP8_E4M3FN: return p.D == 128 ? launch_typed<128, KV_FP8>(p, waves, s) : launch_typed<64, KV_FP8>(p, waves, s);
+    case PA_INT8: return p.D == 128 ? launch_typed<128, KV_I8>(p, waves, s) : launch_typed<64, KV_I8>(p, waves, s);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 void plan_decode_balanced(DecodeParams& p, int num_cus) {
@@ -1418,10 +1481,13 @@ size_t decode_balanced_workspace_bytes(int B, int Hq, int D, int gv) {
 }
 
 hipError_t launch_decode_balanced(const DecodeParams& p, int kv_dtype, hipStream_t s) {
-  const bool fp8 = kv_dtype == PA_FP8_E4M3FN;
-  if (p.D == 128) return fp8 ? launch_balanced_typed<128, true>(p, s) : launch_balanced_typed<128, false>(p, s);
-  if (p.D == 64) return fp8 ? launch_balanced_typed<64, true>(p, s) : launch_balanced_typed<64, false>(p, s);
-  return hipErrorInvalidValue;
+  if (p.D != 64 && p.D != 128) return hipErrorInvalidValue;
+  switch (kv_dtype) {
+    case PA_BF16: return p.D == 128 ? launch_balanced_typed<128, KV_BF16>(p, s) : launch_balanced_typed<64, KV_BF16>(p, s);
+    case PA_FP8_E4M3FN: return p.D == 128 ? launch_balanced_typed<128, KV_FP8>(p, s) : launch_balanced_typed<64, KV_FP8>(p, s);
+    case PA_INT8: return p.D == 128 ? launch_balanced_typed<128, KV_I8>(p, s) : launch_balanced_typed<64, KV_I8>(p, s);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 template <int G>

@@ -9,7 +9,8 @@
 // the way in with one float32 scale per (block, kv head), kept as the running maximum of
 // absmax / 448 over the tokens the block holds: when a write raises the scale, the block's
 // earlier rows are re-encoded under the new one.  A block whose first row is part of the write
-// is fresh (its old scale and contents are ignored).
+// is fresh (its old scale and contents are ignored).  int8 pools keep a scale per (token, kv head) and have a kernel of
+// their own, row by row (kv_write_rows_kernel).
 //
 // One workgroup per (sequence, touched block, kv head, K or V): the (block, head) slab is
 // private to it, so scale maintenance needs no atomics.  Pure streaming work, HBM bound.
@@ -404,14 +405,172 @@ __global__ __launch_bounds__(WGQ) void q_norm_rope_kernel(KvWriteParams p) {
   }
 }
 
+// ---- row-wise write: int8 pools, and packed rows ------------------------------------------------------------
+// int8: a row's scale is its own, s = absmax / 127 (1 for a row of zeros), its codes round(x / s) to nearest even, so
+// a row that has been written is never touched again, whatever is written behind it, and no row needs another's.  That
+// makes the row the unit of work: D / 8 lanes hold one (token, kv head), 16 bytes each of K and of V, and the absmax is
+// a butterfly over them, on the bit patterns: for non-negative floats these order as the values do, and a NaN orders
+// above infinity, so a row that holds either is recognised by the same maximum (its scale becomes NaN and its codes 0:
+// reading it back gives NaN, not a number that looks like data).  The quotient is the correctly rounded one (pa_div.h).
+//
+// A workgroup covers 2^tok_shift consecutive tokens of one sequence for as many kv heads as its lanes leave room for:
+// consecutive tokens of one head come first, because their scales are neighbours in memory (scales
+// [num_blocks, Hkv, block_size]).
+//
+// Packed rows (p.cu): the sequence of a workgroup is found by bisection (packed_find).  bf16 pools take packed rows
+// through the same kernel as plain copies (KIND 2); KIND 1 is int8.
+template <int MASK>
+__device__ __forceinline__ uint32_t butterfly_umax(uint32_t v) {
+  constexpr int ctrl = MASK == 1 ? 0xB1 : MASK == 2 ? 0x4E : MASK == 4 ? 0x141 : 0x140;      // (as butterfly_add)
+  const uint32_t o = MASK <= 8 ? (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true)
+                               : (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, (MASK << 10) | 0x1f);
+  return v > o ? v : o;
+}
+template <int CPR>
+__device__ __forceinline__ uint32_t row_absmax_bits(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = w[j] & 0x7fffu, hi = (w[j] >> 16) & 0x7fffu;
+    m = max(m, max(lo, hi));
+  }
+  if (CPR > 1) m = butterfly_umax<1>(m);
+  if (CPR > 2) m = butterfly_umax<2>(m);
+  if (CPR > 4) m = butterfly_umax<4>(m);
+  if (CPR > 8) m = butterfly_umax<8>(m);
+  if (CPR > 16) m = butterfly_umax<16>(m);
+  return m;
+}
+// eight bf16 values of a row -> eight codes; `amax`: bit pattern of the row's absmax; *scale receives the row's scale
+__device__ __forceinline__ uint2 encode_i8(const uint4& v, uint32_t amax, float* scale) {
+  float s = __fdiv_rn(__uint_as_float(amax << 16), 127.f);
+  if (amax == 0) s = 1.f;
+  if (amax >= 0x7f80u) {
+    *scale = __uint_as_float(0x7fc00000u);
+    return make_uint2(0, 0);
+  }
+  *scale = s;
+  float x[8];
+  unpack8(v, x);
+  if (pa_div_by_ok(s, __float_as_uint(s))) {
+    const float r = pa_refine_rcp(s, __builtin_amdgcn_rcpf(s));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = pa_div_by(x[j], s, r);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = __fdiv_rn(x[j], s);
+  }
+  uint32_t o[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    // (the clamp is for scales so small that absmax / 127 lost bits: their quotients can pass 127)
+    const int c = (int)__builtin_amdgcn_fmed3f(rintf(x[j]), -127.f, 127.f);
+    o[j >> 2] |= (uint32_t)(c & 0xff) << (8 * (j & 3));
+  }
+  return make_uint2(o[0], o[1]);
+}
+
+template <int KIND, int CPR, bool XFORM, bool PACKED>
+__global__ __launch_bounds__(WG) void kv_write_rows_kernel(KvWriteParams p) {
+  constexpr int D = 8 * CPR, ROWS = WG / CPR;
+  const int c = threadIdx.x % CPR, rr = threadIdx.x / CPR;
+  const int tok = rr & ((1 << p.tok_shift) - 1);
+  const int h = blockIdx.y * (ROWS >> p.tok_shift) + (rr >> p.tok_shift);
+  int b, tile;
+  long row0;                                   // row of the sequence's token 0 in k_new / v_new
+  int tq;
+  if (PACKED) {
+    b = packed_find(p.cu, p.B, p.total, p.tok_shift, blockIdx.x, &tile);
+    const int first = packed_row(p.cu, b, p.total);
+    row0 = first;
+    tq = min(p.query_lens[b], packed_row(p.cu, b + 1, p.total) - first);
+  } else {
+    b = blockIdx.z;
+    tile = blockIdx.x;
+    row0 = (long)b * p.T;
+    tq = min(p.query_lens[b], p.T);
+  }
+  const int t = (tile << p.tok_shift) + tok;
+  const int seq = min(p.seq_lens[b], p.max_blocks * p.block_size);
+  const int start = seq - tq;
+  const int pos = start + t;
+  bool live = h < p.Hkv && t >= 0 && t < tq && start >= 0;
+  int blk = -1, in_blk = 0;
+  if (live) {
+    const int jb = pos / p.block_size;
+    in_blk = pos - jb * p.block_size;
+    blk = p.block_tables[(long)b * p.max_blocks + jb];
+    live = blk >= 0 && blk < p.num_blocks;     // a bad table entry must not redirect the write
+  }
+  if (!live) return;                           // whole rows: the lanes of a butterfly stay together
+  const uint4 vraw = *(const uint4*)((const uint16_t*)p.v_new + (row0 + t) * p.v_stride + (long)h * D + 8 * c);
+  uint4 kraw = *(const uint4*)((const uint16_t*)p.k_new + (row0 + t) * p.k_stride + (long)h * D + 8 * c);
+  if (XFORM) {
+    const int rpos = min(pos, p.rope_max_pos - 1);
+    RopeCoeffs<CPR> rc;
+    float wf[8], x[8];
+    rc.load(c, p.rope_cos + (long)rpos * (D / 2), p.rope_sin + (long)rpos * (D / 2));
+    load_norm_weights(p.k_norm_weight, c, wf);
+    unpack8(kraw, x);
+    kraw = norm_rope_chunk<CPR>(x, p.k_norm_weight != nullptr, wf, p.norm_eps, rc);
+  }
+  const long dst = ((long)blk * p.block_size + in_blk) * p.Hkv + h;        // pool row
+  if (KIND == 2) {
+    store_stream((uint16_t*)p.k_cache + dst * D + 8 * c, kraw);
+    store_stream((uint16_t*)p.v_cache + dst * D + 8 * c, vraw);
+    return;
+  }
+  float ks, vs;
+  const uint2 kc = encode_i8(kraw, row_absmax_bits<CPR>(kraw), &ks);
+  const uint2 vc = encode_i8(vraw, row_absmax_bits<CPR>(vraw), &vs);
+  store_stream((uint8_t*)p.k_cache + dst * D + 8 * c, kc);
+  store_stream((uint8_t*)p.v_cache + dst * D + 8 * c, vc);
+  if (c == 0) {
+    const long at = ((long)blk * p.Hkv + h) * p.block_size + in_blk;
+    p.k_scale[at] = ks;
+    p.v_scale[at] = vs;
+  }
+}
+
+template <int KIND, int CPR>
+hipError_t launch_rows(KvWriteParams p, hipStream_t s) {
+  constexpr int ROWS = WG / CPR;
+  // tokens per workgroup: all its rows one head's, fewer when a sequence has fewer new tokens (a decode step: one)
+  const int most = p.cu ? ROWS : p.T;
+  p.tok_shift = 0;
+  while ((1 << p.tok_shift) < most && (1 << p.tok_shift) < ROWS) ++p.tok_shift;
+  const int tt = 1 << p.tok_shift, hh = ROWS / tt;
+  const dim3 grid(p.cu ? p.total / tt + p.B : (p.T + tt - 1) / tt, (p.Hkv + hh - 1) / hh, p.cu ? 1 : p.B);
+  if (p.cu) hipLaunchKernelGGL((kv_write_rows_kernel<KIND, CPR, false, true>), grid, dim3(WG), 0, s, p);
+  else if constexpr (KIND == 1 && CPR >= 8) {
+    if (p.rope_cos) hipLaunchKernelGGL((kv_write_rows_kernel<KIND, CPR, true, false>), grid, dim3(WG), 0, s, p);
+    else hipLaunchKernelGGL((kv_write_rows_kernel<KIND, CPR, false, false>), grid, dim3(WG), 0, s, p);
+  } else hipLaunchKernelGGL((kv_write_rows_kernel<KIND, CPR, false, false>), grid, dim3(WG), 0, s, p);
+  return hipGetLastError();
+}
+template <int KIND>
+hipError_t launch_rows_kind(const KvWriteParams& p, hipStream_t s) {
+  switch (p.D) {
+    case 32: return launch_rows<KIND, 4>(p, s);
+    case 64: return launch_rows<KIND, 8>(p, s);
+    case 128: return launch_rows<KIND, 16>(p, s);
+    case 256: return launch_rows<KIND, 32>(p, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
 template <int CPR>
 void launch_xform(const KvWriteParams& p, dim3 grid, hipStream_t s) {
   if (p.q_in) hipLaunchKernelGGL((q_norm_rope_kernel<CPR, QWG, QUNR>), dim3(p.T, p.B), dim3(QWG), 0, s, p);
+  if (p.kv_dtype == PA_INT8) { (void)launch_rows<1, CPR>(p, s); return; }
   if (p.kv_dtype == PA_FP8_E4M3FN) hipLaunchKernelGGL((kv_write_kernel<1, CPR>), grid, dim3(WG), 0, s, p);
   else hipLaunchKernelGGL((kv_write_kernel<2, CPR>), grid, dim3(WG), 0, s, p);
 }
 
 }  // namespace
+
+bool kv_write_rows_supported(int D) { return D == 32 || D == 64 || D == 128 || D == 256; }
 
 bool kv_write_xform_supported(int D) { return D == 64 || D == 128 || D == 256; }
 
@@ -425,6 +584,8 @@ hipError_t launch_kv_write(const KvWriteParams& p, hipStream_t s) {
     else return hipErrorInvalidValue;
     return hipGetLastError();
   }
+  if (p.kv_dtype == PA_INT8) return launch_rows_kind<1>(p, s);
+  if (p.cu) return p.kv_dtype == PA_BF16 ? launch_rows_kind<2>(p, s) : hipErrorInvalidValue;
   if (p.kv_dtype == PA_FP8_E4M3FN) hipLaunchKernelGGL((kv_write_kernel<1, 0>), grid, dim3(WG), 0, s, p);
   else if (p.kv_dtype == PA_BF16) hipLaunchKernelGGL((kv_write_kernel<2, 0>), grid, dim3(WG), 0, s, p);
   else hipLaunchKernelGGL((kv_write_kernel<4, 0>), grid, dim3(WG), 0, s, p);

@@ -24,8 +24,8 @@ import torch
 
 from . import _lib
 
-F32, BF16, FP8 = 0, 1, 2
-_DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: FP8}
+F32, BF16, FP8, I8 = 0, 1, 2, 4
+_DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: FP8, torch.int8: I8}
 
 _workspaces = {}
 _o_proj_need = {}           # (M, K, N) -> scratch bytes of o_proj's few-rows form (a pure function of the shape)
@@ -102,6 +102,17 @@ def _kv_code(cache, scale_given):
         return FP8
     _check(cache.dtype in _DTYPE_CODE, f"unsupported KV cache dtype {cache.dtype}")
     return _DTYPE_CODE[cache.dtype]
+
+
+def _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, what="KV"):
+    """The scale tables of a pool of codes: one float per (block, kv head) for fp8, per (token, kv head) for int8."""
+    shape, text = ((num_blocks, Hkv), "[num_blocks, Hkv]") if kv_code == FP8 else \
+                  ((num_blocks, Hkv, block_size), "[num_blocks, Hkv, block_size]")
+    _check(k_scale is not None and v_scale is not None,
+           f"{'fp8' if kv_code == FP8 else 'int8'} {what} needs both k_scale and v_scale")
+    for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        _need_device(n, t)
+        _check(t.dtype == torch.float32 and t.shape == shape, f"{n} must be float32 {text}")
 
 
 def _check_paging(k_cache, v_cache, block_tables, seq_lens, B):
@@ -244,11 +255,12 @@ def decode(q, k_cache, v_cache, block_tables, seq_lens, scale, *, k_scale=None, 
 
     q [B, Hq, D] (float32 or bfloat16); k_cache/v_cache [num_blocks, block_size, Hkv, D]
     in q's dtype, or float8_e4m3fn / uint8 codes with k_scale/v_scale [num_blocks, Hkv]
-    float32; block_tables int32 [B, max_blocks]; seq_lens int32 [B].
+    float32, or int8 codes with k_scale/v_scale [num_blocks, Hkv, block_size] (one scale per token and kv head, as
+    `kv_write` leaves them; head_dim 64 or 128, a power-of-two block size >= 16); block_tables int32 [B, max_blocks]; seq_lens int32 [B].
     max_seq_len: host-known upper bound of seq_lens (sizes the split-K grid
     without a device sync; default = table capacity).
     sinks [Hq]: per-head logits that join the softmax as one more column and carry no value;
-    sliding_window W: only the last W keys are visible (bf16 / fp8 pools, head_dim 64 or 128).
+    sliding_window W: only the last W keys are visible (bf16 / fp8 / int8 pools, head_dim 64 or 128).
     q_transform: a `QTransform`; q then holds the rows before norm and rotation (same shapes).
     """
     lib = _lib.load()
@@ -266,16 +278,14 @@ def decode(q, k_cache, v_cache, block_tables, seq_lens, scale, *, k_scale=None, 
     scaled = k_scale is not None or v_scale is not None
     kv_code = _kv_code(k_cache, scaled)
     q_code = _DTYPE_CODE[q.dtype]
-    if kv_code == FP8:
-        _check(q_code == BF16, "fp8 KV needs bfloat16 q")
-        _check(k_scale is not None and v_scale is not None, "fp8 KV needs both k_scale and v_scale")
-        for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need_device(n, t)
-            _check(t.dtype == torch.float32 and t.shape == (num_blocks, Hkv),
-                   f"{n} must be float32 [num_blocks, Hkv]")
+    if kv_code in (FP8, I8):
+        _check(q_code == BF16, f"{'fp8' if kv_code == FP8 else 'int8'} KV needs bfloat16 q")
+        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv)
+        _check(kv_code == FP8 or verify_supported(1, D, block_size),
+               f"int8 KV needs head_dim 64 or 128 and a power-of-two block size >= 16 (D={D}, block_size={block_size})")
     else:
         _check(kv_code == q_code, f"KV dtype {k_cache.dtype} does not match q dtype {q.dtype}")
-        _check(not scaled, "k_scale/v_scale are only valid with an fp8 KV cache")
+        _check(not scaled, "k_scale/v_scale are only valid with an fp8 or int8 KV cache")
     sinks, win = _check_variant(sinks, sliding_window, Hq, q)
     _check(isinstance(partition_size, int) and partition_size > 0, "partition_size must be a positive int")
     cap = block_tables.shape[1] * block_size
@@ -375,7 +385,8 @@ def prefill(q, k_cache, v_cache, block_tables, seq_lens, query_lens, scale, *, k
     matrix-core prefill kernel (head_dim 128, and 64 with two or more kv heads; long query runs
     at head_dim 64 over a single kv head go through the verify kernel 64 tokens at a time).
     `route` = "verify" or "tiled" forces one.  fp8 pools
-    (float8_e4m3fn / uint8 codes with k_scale, v_scale) work on both.  sinks and sliding_window are
+    (float8_e4m3fn / uint8 codes with k_scale, v_scale) work on both; int8 pools on the verify kernel only (longer runs:
+    `read_kv` and `packed_prefill`).  sinks and sliding_window are
     as in `decode`, the window counted back from each query token; so is q_transform, the position of
     row t being seq_lens[b] - query_lens[b] + t.
     max_seq_len: host-known upper bound of seq_lens, as in `decode`; with it a small verify call (a few
@@ -393,22 +404,24 @@ def prefill(q, k_cache, v_cache, block_tables, seq_lens, query_lens, scale, *, k
     _check_paging(k_cache, v_cache, block_tables, seq_lens, B)
     scaled = k_scale is not None or v_scale is not None
     kv_code = _kv_code(k_cache, scaled)
-    _check(kv_code in (BF16, FP8), "prefill needs a bfloat16 or fp8 KV cache")
+    _check(kv_code in (BF16, FP8, I8), "prefill needs a bfloat16, fp8 or int8 KV cache")
     _check(query_lens.shape == (B,) and query_lens.dtype == torch.int32, "query_lens must be int32 [B]")
     num_blocks, block_size, Hkv, Dk = k_cache.shape
     _check(Dk == D, f"head_dim mismatch: q has {D}, cache has {Dk}")
     _check(Hq % Hkv == 0, f"Hq={Hq} is not a multiple of Hkv={Hkv}")
-    if kv_code == FP8:
-        _check(k_scale is not None and v_scale is not None, "fp8 KV needs both k_scale and v_scale")
-        for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need_device(n, t)
-            _check(t.dtype == torch.float32 and t.shape == (num_blocks, Hkv),
-                   f"{n} must be float32 [num_blocks, Hkv]")
+    if kv_code in (FP8, I8):
+        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv)
     else:
-        _check(not scaled, "k_scale/v_scale are only valid with an fp8 KV cache")
+        _check(not scaled, "k_scale/v_scale are only valid with an fp8 or int8 KV cache")
     _check(route in (None, "verify", "tiled"), "route must be None, 'verify' or 'tiled'")
     sinks, win = _check_variant(sinks, sliding_window, Hq, q)
     can_verify = verify_supported(T, D, block_size)
+    if kv_code == I8:
+        # only the decode-shaped kernel reads int8 pools: long query runs read the pool back (read_kv) for packed_prefill
+        _check(route != "tiled" and can_verify,
+               f"prefill over an int8 pool takes runs of up to 64 tokens (the verify kernel: head_dim 64 or 128, a power-of-two "
+               f"block size >= 16; T={T}, D={D}, block_size={block_size}); longer ones go through read_kv and packed_prefill")
+        route = "verify"
     if route is None:
         route = prefill_route(B, T, Hq, Hkv, D, block_size, kv_code == FP8, win,
                               None if max_seq_len is None else int(max_seq_len))
@@ -523,7 +536,29 @@ def gather_kv(cache, block_tables, seq_lens, max_seq_len=None):
     return out
 
 
-def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens, *, k_scale=None, v_scale=None):
+def _token_rows(name, t, dtype=torch.bfloat16):
+    """Packed rows [tokens, heads, D] on the device whose tokens may lie apart (a slice of a wider projection output): the
+    heads and their elements are adjacent, and the token stride is a multiple of 8 elements.  Returns the token stride."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and not t.is_contiguous():
+        _check(t.dim() == 3, f"{name} must be [tokens, heads, D]")
+        _check((t.stride(2) == 1 or t.shape[2] == 1) and (t.stride(1) == t.shape[2] or t.shape[1] == 1),
+               f"{name}: the heads of a token must be adjacent rows of D elements (strides {t.stride()})")
+        _check(t.stride(0) % 8 == 0 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1] * t.shape[2]),
+               f"{name}: the token stride {t.stride(0)} must be a multiple of 8 elements and at least a token's row")
+    else:
+        _need_device(name, t)
+        _check(t.dim() == 3, f"{name} must be [tokens, heads, D]")
+    _check(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
+    _check(t.data_ptr() % 16 == 0, f"{name} must start on a 16-byte boundary")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _check_cu(name, cu, n):
+    _need_device(name, cu)
+    _check(cu.dim() == 1 and cu.dtype == torch.int32 and cu.shape[0] == n + 1, f"{name} must be int32 [{n + 1}]: where each sequence's rows begin")
+
+
+def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens, *, k_scale=None, v_scale=None, cu_seqlens=None):
     """Write the new tokens' K/V into the paged pool, in place, before the attention call.
 
     The reference's `cache_k[:, query_pos] = xk` with query_pos = start_pos + arange(seq_len)
@@ -532,46 +567,121 @@ def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens,
     (block_tables[b, pos // block_size], pos % block_size).  k_new/v_new [B, T, Hkv, D] are
     bfloat16 (float32 for a float32 pool).  float8_e4m3fn pools are quantised on the way in and
     k_scale/v_scale [num_blocks, Hkv] float32 are maintained (running absmax / 448 per block and
-    kv head; earlier rows of a block are re-encoded when its scale grows).  Returns None: the
-    pool tensors are the outputs, aliased to the inputs as the reference's cache tensors are
+    kv head; earlier rows of a block are re-encoded when its scale grows).  int8 pools take codes
+    round(x / s) (nearest even) with s = absmax / 127 of the token's row of a kv head (1 for a row of
+    zeros), kept in k_scale/v_scale [num_blocks, Hkv, block_size] float32: a row's scale is its own, so
+    a written row never changes again (head_dim 32, 64, 128 or 256).  A row that holds an infinity or a NaN
+    gets the scale NaN: it reads back as NaN.
+
+    cu_seqlens int32 [B + 1]: the new rows come packed, k_new/v_new [tokens, Hkv, D] bfloat16 with token t of
+    sequence b in row cu_seqlens[b] + t (bfloat16 and int8 pools); at most the cu_seqlens[b + 1] -
+    cu_seqlens[b] rows of a sequence count, and the rows may be slices of a wider tensor (any token stride that is a
+    multiple of 8 elements).
+
+    Returns None: the pool tensors are the outputs, aliased to the inputs as the reference's cache tensors are
     (examples/models/qwen3/qwen3.py:289-301).
     """
     lib = _lib.load()
-    for n, t in (("k_new", k_new), ("v_new", v_new), ("k_cache", k_cache), ("v_cache", v_cache),
-                 ("block_tables", block_tables), ("seq_lens", seq_lens), ("query_lens", query_lens)):
+    packed = cu_seqlens is not None
+    for n, t in (() if packed else (("k_new", k_new), ("v_new", v_new))) + \
+                (("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens),
+                 ("query_lens", query_lens)):
         _need_device(n, t)
-    _check(k_new.dim() == 4, "k_new must be [B, T, Hkv, D]")
-    _check(v_new.shape == k_new.shape and v_new.dtype == k_new.dtype, "v_new must match k_new")
     _check(k_cache.dim() == 4, "k_cache must be [num_blocks, block_size, Hkv, D]")
     _check(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, "v_cache must match k_cache")
     _check(k_cache.dtype in _DTYPE_CODE, f"unsupported pool dtype {k_cache.dtype}")
-    B, T, Hkv, D = k_new.shape
+    kv_dtype = _DTYPE_CODE[k_cache.dtype]
+    _check(block_tables.dim() == 2 and block_tables.dtype == torch.int32, "block_tables must be int32 [B, max_blocks]")
+    if packed:
+        _check(kv_dtype in (BF16, I8), f"packed rows go into bfloat16 or int8 pools (a float8 pool's scales belong to whole blocks), got {k_cache.dtype}")
+        strides = _token_rows("k_new", k_new), _token_rows("v_new", v_new)
+        B = block_tables.shape[0]
+        _check_cu("cu_seqlens", cu_seqlens, B)
+        Hkv, D = k_new.shape[1:]
+    else:
+        _check(k_new.dim() == 4, "k_new must be [B, T, Hkv, D]")
+        B, T, Hkv, D = k_new.shape
+        want = torch.float32 if kv_dtype == F32 else torch.bfloat16
+        _check(k_new.dtype == want, f"k_new must be {want} for a {k_cache.dtype} pool, got {k_new.dtype}")
+    _check(v_new.shape == k_new.shape and v_new.dtype == k_new.dtype, "v_new must match k_new")
     num_blocks, block_size = k_cache.shape[:2]
     _check(tuple(k_cache.shape[2:]) == (Hkv, D), f"pool rows are {tuple(k_cache.shape[2:])}, new rows {(Hkv, D)}")
-    kv_dtype = _DTYPE_CODE[k_cache.dtype]
-    want = torch.float32 if kv_dtype == F32 else torch.bfloat16
-    _check(k_new.dtype == want, f"k_new must be {want} for a {k_cache.dtype} pool, got {k_new.dtype}")
-    _check(block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.dtype == torch.int32,
-           "block_tables must be int32 [B, max_blocks]")
+    _check(block_tables.shape[0] == B, "block_tables must be int32 [B, max_blocks]")
     _check(seq_lens.shape == (B,) and seq_lens.dtype == torch.int32, "seq_lens must be int32 [B]")
     _check(query_lens.shape == (B,) and query_lens.dtype == torch.int32, "query_lens must be int32 [B]")
-    if kv_dtype == FP8:
-        _check(k_scale is not None and v_scale is not None, "float8 pools need k_scale and v_scale")
-        for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need_device(n, t)
-            _check(t.dtype == torch.float32 and tuple(t.shape) == (num_blocks, Hkv), f"{n} must be float32 [num_blocks, Hkv]")
+    if kv_dtype in (FP8, I8):
+        _check_scales(kv_dtype, k_scale, v_scale, num_blocks, block_size, Hkv, "pool")
     else:
-        _check(k_scale is None and v_scale is None, "k_scale / v_scale are for float8 pools only")
+        _check(k_scale is None and v_scale is None, "k_scale / v_scale are for float8 and int8 pools only")
+    _check(kv_dtype != I8 and not packed or D in (32, 64, 128, 256), f"int8 pools and packed rows need head_dim 32, 64, 128 or 256 (got {D})")
     _same_device(k_new, v_new=v_new, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables,
-                 seq_lens=seq_lens, query_lens=query_lens, k_scale=k_scale, v_scale=v_scale)
+                 seq_lens=seq_lens, query_lens=query_lens, k_scale=k_scale, v_scale=v_scale, cu_seqlens=cu_seqlens)
     with _on(k_new.device):
-        rc = lib.pa_kv_write(_ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache),
-                             _ptr(k_scale) if k_scale is not None else None,
-                             _ptr(v_scale) if v_scale is not None else None,
-                             _ptr(block_tables), _ptr(seq_lens), _ptr(query_lens),
-                             B, T, Hkv, D, block_size, block_tables.shape[1], num_blocks, kv_dtype,
-                             _stream_ptr(k_new.device))
+        if packed:
+            rc = lib.pa_kv_write_packed(_ptr(k_new), _ptr(v_new), *strides, _ptr(cu_seqlens), k_new.shape[0], _ptr(k_cache),
+                                        _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_tables), _ptr(seq_lens),
+                                        _ptr(query_lens), B, Hkv, D, block_size, block_tables.shape[1], num_blocks, kv_dtype,
+                                        _stream_ptr(k_new.device))
+        else:
+            rc = lib.pa_kv_write(_ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache),
+                                 _ptr(k_scale) if k_scale is not None else None,
+                                 _ptr(v_scale) if v_scale is not None else None,
+                                 _ptr(block_tables), _ptr(seq_lens), _ptr(query_lens),
+                                 B, T, Hkv, D, block_size, block_tables.shape[1], num_blocks, kv_dtype,
+                                 _stream_ptr(k_new.device))
     _raise_on(rc, "pa_kv_write")
+
+
+def read_kv(k_cache, v_cache, block_tables, seq_lens, cu_seqlens, total_tokens=None, *, k_scale=None, v_scale=None, out=None):
+    """Read a paged cache back as dense bfloat16 rows: token t < seq_lens[b] of sequence b becomes row cu_seqlens[b] + t of
+    the results (k, v), [total_tokens, Hkv, D] each -- what `packed_prefill` takes as keys and values of a chunk whose
+    first part is cached.
+
+    The block-table gather (np.take of the pool, nkipy/src/nkipy/core/tensor.py:575-640) with the pool's codes
+    multiplied by their scales: int8 pools with k_scale/v_scale [num_blocks, Hkv, block_size], float8_e4m3fn / uint8
+    codes with [num_blocks, Hkv]; bfloat16 pools come out bit for bit.  cu_seqlens int32 [B + 1]; a sequence gets
+    at most cu_seqlens[b + 1] - cu_seqlens[b] rows.  total_tokens: rows of the results, known on the host (at least
+    cu_seqlens[B] for every row to have its place).  out: the pair (k, v) to write into (then total_tokens may be left
+    out); rows on which no token falls are left as they are -- with results allocated here they hold whatever the
+    memory held.
+    """
+    lib = _lib.load()
+    for n, t in (("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens)):
+        _need_device(n, t)
+    _check(block_tables.dim() == 2, "block_tables must be int32 [B, max_blocks_per_seq]")
+    B = block_tables.shape[0]
+    _check_paging(k_cache, v_cache, block_tables, seq_lens, B)
+    num_blocks, block_size, Hkv, D = k_cache.shape
+    scaled = k_scale is not None or v_scale is not None
+    kv_code = _kv_code(k_cache, scaled)
+    _check(kv_code != F32, "read_kv takes bfloat16, float8_e4m3fn / uint8 and int8 pools")
+    if kv_code in (FP8, I8):
+        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, "pool")
+    else:
+        _check(not scaled, "k_scale / v_scale are for float8 and int8 pools only")
+    _check(D % 8 == 0, f"head_dim {D} must be a multiple of 8")
+    _check_cu("cu_seqlens", cu_seqlens, B)
+    if out is None:
+        _check(total_tokens is not None, "total_tokens (rows of the results) is needed without out")
+        N = int(total_tokens)
+        _check(N >= 0, f"total_tokens {N} is negative")
+        out = tuple(torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
+    else:
+        _check(isinstance(out, (tuple, list)) and len(out) == 2, "out must be the pair (k, v)")
+        for n, t in (("out[0]", out[0]), ("out[1]", out[1])):
+            _need_device(n, t)
+            _check(t.dim() == 3 and tuple(t.shape[1:]) == (Hkv, D) and t.dtype == torch.bfloat16 and t.shape[0] == out[0].shape[0],
+                   f"{n} must be bfloat16 [tokens, {Hkv}, {D}]")
+        N = out[0].shape[0]
+        _check(total_tokens is None or int(total_tokens) == N, f"out has {N} rows, total_tokens says {total_tokens}")
+    _same_device(k_cache, v_cache=v_cache, block_tables=block_tables, seq_lens=seq_lens, cu_seqlens=cu_seqlens,
+                 k_scale=k_scale, v_scale=v_scale, k=out[0], v=out[1])
+    with _on(k_cache.device):
+        rc = lib.pa_read_kv(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_tables), _ptr(seq_lens),
+                            _ptr(cu_seqlens), _ptr(out[0]), _ptr(out[1]), N, B, Hkv, D, block_size, block_tables.shape[1],
+                            num_blocks, kv_code, _stream_ptr(k_cache.device))
+    _raise_on(rc, "pa_read_kv")
+    return out[0], out[1]
 
 
 def rope_tables(head_dim: int, max_seq_len: int, base: float = 10000.0, device="cuda"):
@@ -618,7 +728,7 @@ def qk_norm_rope_kv_write(xq, xk, xv, k_cache, v_cache, block_tables, seq_lens, 
     _check(D in (64, 128, 256), f"head_dim {D} must be 64, 128 or 256")
     _check(k_cache.dim() == 4 and tuple(k_cache.shape[2:]) == (Hkv, D), "k_cache must be [num_blocks, block_size, Hkv, D]")
     _check(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, "v_cache must match k_cache")
-    _check(k_cache.dtype in (torch.bfloat16, torch.float8_e4m3fn), f"unsupported pool dtype {k_cache.dtype}")
+    _check(k_cache.dtype in (torch.bfloat16, torch.float8_e4m3fn, torch.int8), f"unsupported pool dtype {k_cache.dtype}")
     num_blocks, block_size = k_cache.shape[:2]
     kv_dtype = _DTYPE_CODE[k_cache.dtype]
     for n, t in (("rope_cos", rope_cos), ("rope_sin", rope_sin)):
@@ -632,13 +742,10 @@ def qk_norm_rope_kv_write(xq, xk, xv, k_cache, v_cache, block_tables, seq_lens, 
            "block_tables must be int32 [B, max_blocks]")
     _check(seq_lens.shape == (B,) and seq_lens.dtype == torch.int32, "seq_lens must be int32 [B]")
     _check(query_lens.shape == (B,) and query_lens.dtype == torch.int32, "query_lens must be int32 [B]")
-    if kv_dtype == FP8:
-        _check(k_scale is not None and v_scale is not None, "float8 pools need k_scale and v_scale")
-        for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need_device(n, t)
-            _check(t.dtype == torch.float32 and tuple(t.shape) == (num_blocks, Hkv), f"{n} must be float32 [num_blocks, Hkv]")
+    if kv_dtype in (FP8, I8):
+        _check_scales(kv_dtype, k_scale, v_scale, num_blocks, block_size, Hkv, "pool")
     else:
-        _check(k_scale is None and v_scale is None, "k_scale / v_scale are for float8 pools only")
+        _check(k_scale is None and v_scale is None, "k_scale / v_scale are for float8 and int8 pools only")
     if xq is not None:
         if out is None:
             out = torch.empty_like(xq)
@@ -787,15 +894,14 @@ def prepare_decode_step(xq, xk, xv, k_cache, v_cache, block_tables, seq_lens, qu
     scaled = k_scale is not None or v_scale is not None
     kv_code = _kv_code(k_cache, scaled)
     q_code = _DTYPE_CODE[xq.dtype]
-    if kv_code == FP8:
-        _check(q_code == BF16, "fp8 KV needs bfloat16 rows")
-        _check(k_scale is not None and v_scale is not None, "fp8 KV needs both k_scale and v_scale")
-        for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need_device(n, t)
-            _check(t.dtype == torch.float32 and t.shape == (num_blocks, Hkv), f"{n} must be float32 [num_blocks, Hkv]")
+    if kv_code in (FP8, I8):
+        _check(q_code == BF16, f"{'fp8' if kv_code == FP8 else 'int8'} KV needs bfloat16 rows")
+        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv)
+        _check(kv_code == FP8 or verify_supported(1, D, block_size),
+               f"int8 KV needs head_dim 64 or 128 and a power-of-two block size >= 16 (D={D}, block_size={block_size})")
     else:
         _check(kv_code == q_code, f"KV dtype {k_cache.dtype} does not match the rows' dtype {xq.dtype}")
-        _check(not scaled, "k_scale/v_scale are only valid with an fp8 KV cache")
+        _check(not scaled, "k_scale/v_scale are only valid with an fp8 or int8 KV cache")
     sinks, win = _check_variant(sinks, sliding_window, Hq, xq)
     _check(isinstance(partition_size, int) and partition_size > 0, "partition_size must be a positive int")
     cap = block_tables.shape[1] * block_size
@@ -897,14 +1003,11 @@ def prepare_verify_step(xq, xk, xv, k_cache, v_cache, block_tables, seq_lens, qu
     _check(query_lens.shape == (B,) and query_lens.dtype == torch.int32, "query_lens must be int32 [B]")
     scaled = k_scale is not None or v_scale is not None
     kv_code = _kv_code(k_cache, scaled)
-    _check(kv_code in (BF16, FP8), "verify_step needs a bfloat16 or fp8 KV cache")
-    if kv_code == FP8:
-        _check(k_scale is not None and v_scale is not None, "fp8 KV needs both k_scale and v_scale")
-        for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need_device(n, t)
-            _check(t.dtype == torch.float32 and t.shape == (num_blocks, Hkv), f"{n} must be float32 [num_blocks, Hkv]")
+    _check(kv_code in (BF16, FP8, I8), "verify_step needs a bfloat16, fp8 or int8 KV cache")
+    if kv_code in (FP8, I8):
+        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv)
     else:
-        _check(not scaled, "k_scale/v_scale are only valid with an fp8 KV cache")
+        _check(not scaled, "k_scale/v_scale are only valid with an fp8 or int8 KV cache")
     sinks, win = _check_variant(sinks, sliding_window, Hq, xq)
     cap = block_tables.shape[1] * block_size
     msl = 0 if max_seq_len is None else int(max_seq_len)
