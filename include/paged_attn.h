@@ -226,6 +226,34 @@ int pa_prefill(const void* q, const void* k_cache, const void* v_cache,
                void* workspace, size_t workspace_bytes, const pa_q_transform* q_transform, void* stream);
 
 /*
+ * Causal attention over whole prompts of different lengths, packed row behind row, with dense K and V: what
+ * pa_prefill computes on a paged pool, for keys and values that are at hand as rows -- the projections' own output (a
+ * prompt without a cached prefix), or a cache read back by pa_read_kv (examples/models/qwen3/kernels/attention.py:112-144
+ * per sequence; with keys in front of the queries gpt_oss/kernels/attention.py:85,127-135).
+ *   q [total_q, Hq, D], k, v [total_k, Hkv, D], out [total_q, Hq, D] (contiguous)  bf16, D 64 or 128; consecutive tokens
+ *                 of q, k and v lie q_stride, k_stride, v_stride elements apart (multiples of 8, at least a
+ *                 token's row): slices of a wider tensor
+ *   cu_seqlens_q, cu_seqlens_k [num_seqs + 1]  sequence i's rows are cu[i] .. cu[i + 1] - 1 of q / out, and of k / v
+ *                 (both may be the same array); boundaries outside [0, total] count as its ends
+ *   query_lens, seq_lens [num_seqs] or NULL    of those rows, the first query_lens[i] are queries (the others are
+ *                 padding, zero in out) and the first seq_lens[i] are keys (the others are never read)
+ *   query t of a sequence of n queries and c keys sees keys j <= c - n + t: the last query sees them all; a query
+ *                 that sees no key (c < n) gets zeros
+ *   out           rows that belong to no sequence are left as they are
+ *   sinks, sliding_window   as for pa_prefill, for both head dims
+ *   max_seq_len   0, or a host-known upper bound of a sequence's keys (a hint: see the workspace)
+ *   workspace     NULL, or pa_packed_prefill_workspace_bytes(...) bytes (16-byte aligned; 0 = none needed): with it, a
+ *                 call of few queries over many keys splits the keys of a query tile over several workgroups and merges
+ *                 their results in a second kernel
+ */
+size_t pa_packed_prefill_workspace_bytes(int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len);
+int pa_packed_prefill(const void* q, const void* k, const void* v, long q_stride, long k_stride, long v_stride,
+                      const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* query_lens,
+                      const int32_t* seq_lens, void* out, void* workspace, size_t workspace_bytes,
+                      int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len,
+                      float scale, int dtype, const float* sinks, int sliding_window, void* stream);
+
+/*
  * Block-sparse causal prefill over dense q [B, S, Hq, D], k/v [B, S, Hkv, D]:
  * q block i attends k block j iff j <= i and (i - j < local_blocks or
  * (j + h % vert_stride) % vert_stride == 0), token-causal inside a block.

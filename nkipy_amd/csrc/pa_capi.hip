@@ -938,6 +938,74 @@ int pa_prefill(const void* q, const void* k_cache, const void* v_cache,
   return check_hip(e, "pa_prefill launch");
 }
 
+static void fill_packed_shape(PrefillParams& p, int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len) {
+  memset(&p, 0, sizeof(p));
+  p.B = num_seqs; p.total_q = total_q; p.total_k = total_k; p.Hq = Hq; p.Hkv = Hkv; p.D = D;
+  p.block_shift = -1;
+  p.len_bound = max_seq_len;
+  p.impl = g_prefill_impl.load();
+  p.num_cus = current_num_cus();
+}
+
+size_t pa_packed_prefill_workspace_bytes(int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len) {
+  if (num_seqs <= 0 || total_q <= 0 || total_k <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (D != 64 && D != 128) ||
+      (long)total_q * (Hq / Hkv) + num_seqs > 0x7fff0000L)
+    return 0;
+  PrefillParams p;
+  fill_packed_shape(p, num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len);
+  const int want = prefill_packed_splits(p, p.num_cus);
+  return want > 1 ? (size_t)total_q * Hq * want * ((size_t)D + 2) * sizeof(float) : 0;
+}
+
+int pa_packed_prefill(const void* q, const void* k, const void* v, long q_stride, long k_stride, long v_stride,
+                      const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* query_lens,
+                      const int32_t* seq_lens, void* out, void* workspace, size_t workspace_bytes,
+                      int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len,
+                      float scale, int dtype, const float* sinks, int sliding_window, void* stream) {
+  tl_error[0] = 0;
+  const char* who = "pa_packed_prefill";
+  if (num_seqs < 0 || total_q < 0 || total_k < 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return fail_arg("%s: bad sizes", who);
+  if (Hq % Hkv) return fail_arg("%s: Hq=%d is not a multiple of Hkv=%d", who, Hq, Hkv);
+  if (dtype != PA_BF16) return fail_arg("%s: only bf16 is supported (dtype=%d)", who, dtype);
+  if (D != 64 && D != 128) return fail_arg("%s: head_dim %d must be 64 or 128", who, D);
+  if (sliding_window < 0) return fail_arg("%s: sliding_window=%d must be >= 0 (0 = none)", who, sliding_window);
+  if (max_seq_len < 0) return fail_arg("%s: max_seq_len=%d must be >= 0 (0 = not known)", who, max_seq_len);
+  const long qrow = (long)Hq * D, krow = (long)Hkv * D;
+  if (q_stride < qrow || k_stride < krow || v_stride < krow || q_stride % 8 || k_stride % 8 || v_stride % 8)
+    return fail_arg("%s: token strides (%ld, %ld, %ld elements) must be multiples of 8 and at least a token's row (%ld, %ld)", who,
+                    q_stride, k_stride, v_stride, qrow, krow);
+  // (byte offsets within four rows are 32-bit in the kernel, row numbers times heads 31-bit)
+  if (k_stride > 0x0fffffffL || v_stride > 0x0fffffffL) return fail_arg("%s: a token stride exceeds 2^28 elements", who);
+  if ((long)total_q * (Hq / Hkv) + num_seqs > 0x7fff0000L)
+    return fail_arg("%s: %d rows of %d q heads per kv head exceed 2^31", who, total_q, Hq / Hkv);
+  if (num_seqs == 0 || total_q == 0) return 0;
+  if (!q || !cu_seqlens_q || !out || (total_k > 0 && (!k || !v)) || !cu_seqlens_k) return fail_arg("%s: null pointer argument", who);
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return fail_arg("%s: q, k, v and out must be 16-byte aligned", who);
+  if (!aligned16(workspace)) return fail_arg("%s: workspace must be 16-byte aligned", who);
+  PrefillParams p;
+  fill_packed_shape(p, num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len);
+  p.q = q; p.k = k; p.v = v; p.out = out;
+  p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.query_lens = query_lens; p.seq_lens = seq_lens;
+  p.q_stride = q_stride; p.k_stride = k_stride; p.v_stride = v_stride;
+  p.scale_log2e = scale * kLog2e;
+  p.sinks = sinks; p.window = sliding_window;
+  p.splits = 1;
+  if (workspace) {
+    const int forced = g_prefill_split.load();       // 1: the rule; 0: never; 2-16: that many shares
+    const int want = forced == 1 ? prefill_packed_splits(p, p.num_cus) : forced <= 0 ? 1 : std::min(forced, 16);
+    if (want > 1 && workspace_bytes >= (size_t)total_q * Hq * want * ((size_t)D + 2) * sizeof(float)) {
+      p.splits = want;
+      p.ws_o = (float*)workspace;
+      p.ws_ml = p.ws_o + (size_t)total_q * Hq * want * D;
+    }
+  }
+  hipStream_t s = (hipStream_t)stream;
+  profile_begin(s);
+  hipError_t e = launch_prefill_packed(p, s);
+  profile_end(s);
+  return check_hip(e, "pa_packed_prefill launch");
+}
+
 int pa_blocksparse_prefill(const void* q, const void* k, const void* v, void* out,
                            int B, int S, int Hq, int Hkv, int D,
                            int block, int local_blocks, int vert_stride,

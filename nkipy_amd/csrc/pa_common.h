@@ -92,20 +92,24 @@ template <> struct Store<uint16_t> {
 };
 
 // ---- packed rows -------------------------------------------------------------------
-// Sequence i of n owns rows [cu[i], cu[i + 1]) of a packed tensor of `total` rows.  Work is dealt in tiles of 2^shift rows
-// of one sequence; tile t of sequence i has the number floor(cu[i] / 2^shift) + i + t, which no other tile has and
-// which needs no pass over the lengths: from one sequence to the next it grows by floor(cu[i + 1] / 2^shift) -
-// floor(cu[i] / 2^shift) + 1 >= ceil(len / 2^shift).  So floor(total / 2^shift) + n numbers cover every tile (some have
-// none), and the sequence of a number is found by bisection.  Boundaries outside [0, total] count as its ends.
-__device__ __forceinline__ int packed_row(const int32_t* cu, int i, int total) { return min(max(cu[i], 0), total); }
-__device__ __forceinline__ int packed_find(const int32_t* cu, int n, int total, int shift, int slot, int* tile) {
-  int lo = 0, hi = n;                     // the last i with first_slot(i) <= slot lies in [lo, hi)
+// Sequence i of n owns rows [cu[i], cu[i + 1]) of a packed tensor of `total` rows.  Work is dealt in tiles of 2^shift
+// units of one sequence, a row being `mult` units; tile t of sequence i has the number floor(mult cu[i] / 2^shift) + i + t,
+// which no other tile has and which needs no pass over the lengths: from one sequence to the next it grows by
+// floor(mult cu[i + 1] / 2^shift) - floor(mult cu[i] / 2^shift) + 1 >= ceil(mult len / 2^shift).  So
+// floor(mult total / 2^shift) + n numbers cover every tile (some have none), and the sequence of a number is found by
+// bisection.  Boundaries outside [0, total] count as its ends; mult * total is below 2^31 (checked on the host).
+// (Wave-uniform indices through the constant address space are scalar loads.)
+typedef const __attribute__((address_space(4))) int32_t* packed_ptr;
+__device__ __forceinline__ packed_ptr as_packed(const int32_t* cu) { return (packed_ptr)(uintptr_t)cu; }
+__device__ __forceinline__ int packed_row(packed_ptr cu, int i, int total) { return min(max(cu[i], 0), total); }
+__device__ __forceinline__ int packed_find(packed_ptr cu, int n, int total, int shift, int slot, int* tile, int mult = 1) {
+  int lo = 0, hi = n;                     // the last i whose first number is not above slot lies in [lo, hi)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if ((packed_row(cu, mid, total) >> shift) + mid <= slot) lo = mid;
+    if (((mult * packed_row(cu, mid, total)) >> shift) + mid <= slot) lo = mid;
     else hi = mid;
   }
-  *tile = slot - ((packed_row(cu, lo, total) >> shift) + lo);
+  *tile = slot - (((mult * packed_row(cu, lo, total)) >> shift) + lo);
   return lo;
 }
 
@@ -292,6 +296,13 @@ struct PrefillParams {
   float* ws_o;              // splits > 1: [B * T * Hq, splits, D] partial outputs
   float* ws_ml;             // splits > 1: [B * T * Hq, splits, 2] partial (max, sum)
   QTransform qt;            // asynchronous kernel only: Q rows are normed and rotated as they are loaded
+  // packed form (cu_q set; B sequences, no block tables): sequence b's queries are rows cu_q[b] .. of q / out, its keys
+  // rows cu_k[b] .. of k / v; of them the first query_lens[b] / seq_lens[b] count (null: all)
+  const int32_t* cu_q;      // [B + 1]
+  const int32_t* cu_k;
+  int total_q, total_k;     // rows of q and of k / v
+  long q_stride, k_stride, v_stride;    // elements from one token to the next
+  int slots;                // query tiles are numbered 0 .. slots - 1 (packed_find)
   int num_cus;              // CUs of the device the call runs on (0: unknown, taken as 256); steers the workgroup shape
   int len_bound;            // the caller's bound on the sequence lengths (0: none); steers the workgroup shape as well
 };
@@ -301,6 +312,8 @@ int prefill_async_splits(const PrefillParams& p, int num_cus, int max_seq_len = 
 bool prefill_supported(const PrefillParams& p);
 hipError_t launch_prefill_async(const PrefillParams& p, int waves, hipStream_t s);
 bool prefill_async_supported(const PrefillParams& p);
+int prefill_packed_splits(const PrefillParams& p, int num_cus);       // packed form: shares of a query tile's keys the launcher would like
+hipError_t launch_prefill_packed(const PrefillParams& p, hipStream_t s);
 
 // ---- gather ------------------------------------------------------------------------
 // ---- paged KV write --------------------------------------------------------------

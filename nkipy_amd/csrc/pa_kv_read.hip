@@ -20,9 +20,9 @@ template <int KV>      // pool type: PA_BF16, PA_FP8_E4M3FN, PA_INT8
 __global__ __launch_bounds__(WG) void kv_read_kernel(KvReadParams p) {
   constexpr int EB = KV == PA_BF16 ? 2 : 1;
   int tile;
-  const int b = packed_find(p.cu, p.B, p.total, TOK_SHIFT, blockIdx.x, &tile);
-  const int first = packed_row(p.cu, b, p.total);
-  const int n = min(min(p.seq_lens[b], p.max_blocks * p.block_size), packed_row(p.cu, b + 1, p.total) - first);
+  const int b = packed_find(as_packed(p.cu), p.B, p.total, TOK_SHIFT, blockIdx.x, &tile);
+  const int first = packed_row(as_packed(p.cu), b, p.total);
+  const int n = min(min(p.seq_lens[b], p.max_blocks * p.block_size), packed_row(as_packed(p.cu), b + 1, p.total) - first);
   const int t0 = tile << TOK_SHIFT;
   if (tile < 0 || t0 >= n) return;
   const bool is_v = blockIdx.y != 0;

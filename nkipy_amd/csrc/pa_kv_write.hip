@@ -481,10 +481,10 @@ __global__ __launch_bounds__(WG) void kv_write_rows_kernel(KvWriteParams p) {
   long row0;                                   // row of the sequence's token 0 in k_new / v_new
   int tq;
   if (PACKED) {
-    b = packed_find(p.cu, p.B, p.total, p.tok_shift, blockIdx.x, &tile);
-    const int first = packed_row(p.cu, b, p.total);
+    b = packed_find(as_packed(p.cu), p.B, p.total, p.tok_shift, blockIdx.x, &tile);
+    const int first = packed_row(as_packed(p.cu), b, p.total);
     row0 = first;
-    tq = min(p.query_lens[b], packed_row(p.cu, b + 1, p.total) - first);
+    tq = min(p.query_lens[b], packed_row(as_packed(p.cu), b + 1, p.total) - first);
   } else {
     b = blockIdx.z;
     tile = blockIdx.x;

@@ -92,7 +92,8 @@ __device__ __forceinline__ void dma16_lane_stream(const char* addr, uint32_t lds
 // waited for in order with the copies above.
 typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
 
-// MODE: 0 = dense K/V [B, S, Hkv, D]; 1 = paged, block size a power of two >= 16.
+// MODE: 0 = dense K/V [B, S, Hkv, D]; 1 = paged, block size a power of two >= 16; 2 = packed: sequences of different
+// lengths row behind row, dense K/V (p.cu_q, p.cu_k).
 // TT: 32-key sub-tiles per key tile (2: 64-key tiles).
 // PACK (short chunks of a GQA model): the query rows of a workgroup are (token, head) pairs of one
 // kv head, token-major, instead of 32*NW tokens of one q head: a chunk of T < 32*NW tokens then fills
@@ -130,7 +131,9 @@ void prefill_async_kernel(PrefillParams p) {
   // a partner: its workgroups take the 256 bytes that end with it (the pair one head earlier), the second half
   // of the waves works for it and the first half only copies (`idle_half`).
   constexpr bool PAIR = DH == 64;
-  static_assert(DH == HD || (PAIR && NW == 8 && MODE == 1 && !SPARSE && !PACK), "head dim 64: 8-wave paged dense form only");
+  constexpr bool PACKED = MODE == 2;
+  static_assert(DH == HD || (PAIR && NW == 8 && MODE != 0 && !SPARSE && !PACK), "head dim 64: 8-wave paged or packed form only");
+  static_assert(!PACKED || (!SPARSE && !FP8), "packed form: plain causal attention over bf16 rows");
   static_assert(QH == 1 || (QH == 2 && PAIR), "two q heads per wave: head dim 64 only");
   constexpr int KS = DH / 16;                // k-steps of the score product
   constexpr int VC = DH / 32;                // 32-wide d chunks of the output
@@ -160,49 +163,101 @@ void prefill_async_kernel(PrefillParams p) {
   const int n_rep = p.Hq / p.Hkv;
   const int nqt = PACK ? (p.T * n_rep + BMW - 1) / BMW : (p.T + TOKW - 1) / TOKW;
   const int kvg = PAIR ? (p.Hkv + 1) / 2 : p.Hkv;    // K/V row groups: kv heads, or pairs of them
-  const int hpg = n_rep / QH;                  // workgroups (per query tile) that cover the q heads of a kv head
-  const int per_group = PACK ? nqt : nqt * hpg;
-  // PACK with one row tile per kv head: this workgroup is the only reader of its keys and values
-  const bool stream_kv = PACK && nqt == 1;
-  const int groups = p.B * kvg;
-  const int xcd = blockIdx.x & 7;
+  // Packed form over a single kv head of 64: there is no second head for the other half of a 256-byte row; both halves
+  // of the tile hold that head (`solo`), and the two halves of the waves work for different q heads of it.
+  const bool solo = PACKED && PAIR && p.Hkv == 1;
+  const int units = n_rep / QH;                // q heads (or pairs of them) of a kv head
+  const int hpg = solo ? (units + 1) / 2 : units;    // workgroups (per query tile) that cover the q heads of a kv head
   const int part = SPLIT ? (int)(blockIdx.x >> 3) % p.splits : 0;      // which share of the key tiles
   const int slot = SPLIT ? (int)(blockIdx.x >> 3) / p.splits : (int)(blockIdx.x >> 3);
-  const int grp = xcd + 8 * (slot / per_group);
-  if (grp >= groups) return;
-  const int rr_ = slot % per_group;
-  const int b = grp / kvg, hk = grp % kvg;     // PAIR: hk numbers the pair
-  const int qt = PACK ? nqt - 1 - rr_ : nqt - 1 - rr_ / hpg;
-  const int kv0 = PAIR ? min(2 * hk, p.Hkv - 2) : hk;    // first kv head of the rows' 256 bytes (PAIR: Hkv >= 2, checked on the host)
+  const int xcd = blockIdx.x & 7;
+  int b, hk, rr_, qt;                          // sequence, kv head (PAIR: pair of them), q head (pair) of the group, query tile
+  bool stream_kv;                              // PACK with one row tile per kv head: the only reader of its keys and values
+  int seg, q_first, k_first, seg_k;            // packed: rows of the sequence and its first row, in q and in k / v
+  if constexpr (PACKED) {
+    // All kv heads have the same work, so they are dealt over the XCDs: with a multiple of eight heads each XCD has its
+    // own ones, with one, two or four several XCDs share a head's query tiles, and any other number takes the heads in
+    // turn.  The q heads of a tile come next to one another.
+    int rest;
+    if (kvg % 8 == 0) {
+      const int per_head = p.slots * (PACK ? 1 : hpg);
+      hk = xcd + 8 * (slot / per_head);
+      rest = slot % per_head;
+    } else if (8 % kvg == 0) {
+      hk = xcd % kvg;
+      rest = slot * (8 / kvg) + xcd / kvg;
+    } else {
+      const int item = slot * 8 + xcd;
+      hk = item % kvg;
+      rest = item / kvg;
+    }
+    if (hk >= kvg) return;
+    const int number = PACK ? rest : rest / hpg;
+    rr_ = PACK ? 0 : rest % hpg;
+    if (number >= p.slots) return;
+    constexpr int SHIFT = (TOKW == 256 ? 8 : 7);
+    static_assert(TOKW == 256 || TOKW == 128, "query tiles of 128 or 256 rows");
+    const int mult = PACK ? n_rep : 1;
+    int tile;
+    b = packed_find(as_packed(p.cu_q), p.B, p.total_q, SHIFT, number, &tile, mult);
+    q_first = packed_row(as_packed(p.cu_q), b, p.total_q);
+    seg = packed_row(as_packed(p.cu_q), b + 1, p.total_q) - q_first;
+    k_first = packed_row(as_packed(p.cu_k), b, p.total_k);
+    seg_k = max(packed_row(as_packed(p.cu_k), b + 1, p.total_k) - k_first, 0);
+    const int tiles = (seg * mult + TOKW - 1) >> SHIFT;
+    if (tile < 0 || tile >= tiles) return;
+    qt = tiles - 1 - tile;                     // the tiles with the most keys first
+    stream_kv = PACK && tiles == 1;
+  } else {
+    const int per_group = PACK ? nqt : nqt * hpg;
+    stream_kv = PACK && nqt == 1;
+    const int groups = p.B * kvg;
+    const int grp = xcd + 8 * (slot / per_group);
+    if (grp >= groups) return;
+    rr_ = slot % per_group;
+    b = grp / kvg, hk = grp % kvg;
+    qt = PACK ? nqt - 1 - rr_ : nqt - 1 - rr_ / hpg;
+    seg = p.T; q_first = 0; k_first = 0; seg_k = 0;
+  }
+  const int kv0 = PAIR ? max(min(2 * hk, p.Hkv - 2), 0) : hk;    // first kv head of the rows' 256 bytes (PAIR: Hkv >= 2, checked on the host, but for `solo`)
   const int hq = PACK ? hk * n_rep : kv0 * n_rep + QH * (rr_ % hpg);     // PACK: first head of the group; PAIR: the first kv head's; QH 2: and hq + 1
+  const int half_heads = solo ? QH * hpg : n_rep;      // PAIR: q heads between the two halves' waves
   // row r of the workgroup (0 .. BMW-1) -> query token and q head
   const int v0 = qt * TOKW;
   auto row_token = [&](int r) __attribute__((always_inline)) { return PACK ? (v0 + r) / n_rep : v0 + (PAIR ? (r & (TOKW - 1)) : r); };
-  auto row_head = [&](int r) __attribute__((always_inline)) { return PACK ? hq + (v0 + r) % n_rep : hq + (PAIR && r >= TOKW ? n_rep : 0); };
+  auto row_head = [&](int r) __attribute__((always_inline)) { return PACK ? hq + (v0 + r) % n_rep : hq + (PAIR && r >= TOKW ? half_heads : 0); };
   const int par = PAIR ? wave / (NW / 2) : 0;   // which 128 bytes of the rows this wave works on
-  const bool lone = PAIR && 2 * hk + 1 >= p.Hkv;          // the unpaired last head of an odd Hkv
-  const bool idle_half = lone && par == 0;                // these waves' head belongs to the pair before: copies only
+  const bool lone = PAIR && !solo && 2 * hk + 1 >= p.Hkv;     // the unpaired last head of an odd Hkv
+  const bool solo_odd = solo && rr_ + hpg >= units;           // ... or an odd number of q heads (pairs) of a single kv head
+  const bool idle_half = (lone && par == 0) || (solo_odd && par == 1);    // these waves only copy: their head belongs to another workgroup, or is none
+  auto row_idle = [&](int r) __attribute__((always_inline)) { return PAIR && ((lone && r < TOKW) || (solo_odd && r >= TOKW)); };
+  // row of a query token in q and out
+  auto token_row = [&](int t) __attribute__((always_inline)) -> long { return PACKED ? (long)q_first + t : (long)b * p.T + t; };
 
-  int tq = p.query_lens ? p.query_lens[b] : p.T;
-  int ctx = p.seq_lens ? p.seq_lens[b] : p.S;
-  tq = min(max(tq, 0), p.T);
-  if (MODE != 0) ctx = min(ctx, p.max_blocks * p.block_size);
+  int tq = p.query_lens ? p.query_lens[b] : seg;
+  int ctx = p.seq_lens ? p.seq_lens[b] : PACKED ? seg_k : p.S;
+  tq = min(max(tq, 0), seg);
+  if (MODE == 1) ctx = min(ctx, p.max_blocks * p.block_size);
+  if (PACKED) ctx = min(ctx, seg_k);
   ctx = max(ctx, 0);
-  tq = min(tq, ctx);          // more query tokens than context: the first ctx of them count, without a prefix (as pa_verify)
+  // more query tokens than context: the first ctx of them count, without a prefix (as pa_verify); packed rows keep the
+  // alignment of the last query with the last key, and the first tq - ctx of them see nothing
+  if (!PACKED) tq = min(tq, ctx);
   const int prefix = ctx - tq;
   const int q0 = row_token(0);                                    // first query token of the workgroup
   uint16_t* out = (uint16_t*)p.out;
   const long q_row_stride = (long)p.Hq * DH;
 
-  if (q0 >= tq) {   // only padding rows here: zeros (written by the reduce kernel when splitting)
+  const int k_end = prefix + min(row_token(BMW - 1) + 1, tq);     // keys the workgroup needs: [0, k_end)
+  if (q0 >= tq || (PACKED && k_end <= 0)) {   // only padding rows here, or rows that see no key: zeros (written by the reduce kernel when splitting)
     if (SPLIT) return;
     for (int i = tid; i < BMW * (DH / 8); i += NW * 64) {
       const int r = i / (DH / 8);
       const int row = row_token(r);
-      if (row < p.T && !(lone && r < TOKW)) {
+      if (row < seg && !row_idle(r)) {
 #pragma unroll
         for (int j = 0; j < QH; ++j)
-          *(uint4*)(out + ((long)b * p.T + row) * q_row_stride + (long)(row_head(r) + j) * DH + (i % (DH / 8)) * 8) = make_uint4(0, 0, 0, 0);
+          *(uint4*)(out + token_row(row) * q_row_stride + (long)(row_head(r) + j) * DH + (i % (DH / 8)) * 8) = make_uint4(0, 0, 0, 0);
       }
     }
     return;
@@ -218,14 +273,13 @@ void prefill_async_kernel(PrefillParams p) {
   const int wq_lo = row_token(wave * 32);                         // first token of this wave
   const int wq_hi = min(row_token(wave * 32 + 31), tq - 1);       // last valid token (may be < wq_lo)
   const bool wave_has_rows = wq_lo < tq && !idle_half;
-  const int k_end = prefix + min(row_token(BMW - 1) + 1, tq);     // keys the workgroup needs: [0, k_end)
   // sliding window (its own instantiation, so that the plain form carries none of its scalar
   // work): the row at position pos sees keys (pos - win, pos]
   const int win = WIN ? p.window : 0;
   // key tiles of this workgroup: [kt_begin, ntiles)
   int kt_begin = win > 0 ? max(prefix + q0 - win + 1, 0) / BN : 0;   // first tile the first row sees
   int ntiles = (k_end + BN - 1) / BN;
-  const long row_g = ((long)b * p.T + qrow) * p.Hq + hq_l;            // this lane's (first) row among all B * T * Hq
+  const long row_g = token_row(qrow) * p.Hq + hq_l;                   // this lane's (first) row among all tokens x heads
   if (SPLIT) {
     const int n_all = ntiles - kt_begin;
     const int lo = kt_begin + (int)((long)part * n_all / p.splits);
@@ -243,26 +297,29 @@ void prefill_async_kernel(PrefillParams p) {
   // A tile is 2 UK units of 1 KB (4 rows): the first UK are K, the rest V.  Wave w issues
   // units w, w + NW, ...  In a unit lane i fills LDS slot (row 4u + i/16, position i%16)
   // with the global chunk  position ^ (row & 7).
-  const const_i32_ptr table = MODE != 0 ? (const_i32_ptr)(uintptr_t)(p.block_tables + (long)b * p.max_blocks) : nullptr;
+  const const_i32_ptr table = MODE == 1 ? (const_i32_ptr)(uintptr_t)(p.block_tables + (long)b * p.max_blocks) : nullptr;
   const uint32_t smem_base = (uint32_t)(uintptr_t)(lds_char*)smem;
-  const long kv_row_bytes = (long)p.Hkv * DH * EB;
-  const char* kbase = (const char*)p.k + (long)kv0 * DH * EB;    // PAIR: 256 bytes from kv head kv0 on
-  const char* vbase = (const char*)p.v + (long)kv0 * DH * EB;
+  const long kv_row_bytes = PACKED ? p.k_stride * EB : (long)p.Hkv * DH * EB;
+  const long v_row_bytes = PACKED ? p.v_stride * EB : kv_row_bytes;
+  const char* kbase = (const char*)p.k + (long)kv0 * DH * EB + (PACKED ? k_first * kv_row_bytes : 0);    // PAIR: 256 bytes from kv head kv0 on
+  const char* vbase = (const char*)p.v + (long)kv0 * DH * EB + (PACKED ? k_first * v_row_bytes : 0);
   const int dma_rr = lane >> 4, dma_pos = lane & 15;
   // every unit of a wave starts at the same row modulo 16 (NW is a multiple of 4), hence the
   // same swizzle: K rows use row & 15, V rows 4 * (row & 3) (what their read patterns want)
-  const int dma_chunk_k = dma_pos ^ ((4 * (wave & 3) + dma_rr) & 15);
-  const int dma_chunk_v = dma_pos ^ (4 * dma_rr);
+  const int solo_mask = solo ? 7 : 15;         // (solo: the chunks of the one head, twice)
+  const int dma_chunk_k = (dma_pos ^ ((4 * (wave & 3) + dma_rr) & 15)) & solo_mask;
+  const int dma_chunk_v = (dma_pos ^ (4 * dma_rr)) & solo_mask;
   const uint32_t kv_row_bytes_u = (uint32_t)kv_row_bytes;
-  const uint32_t block_bytes_u = MODE != 0 ? (uint32_t)p.block_size * kv_row_bytes_u : 0u;
+  const uint32_t block_bytes_u = MODE == 1 ? (uint32_t)p.block_size * kv_row_bytes_u : 0u;
   const int dma_lane_off_k = (int)(dma_rr * kv_row_bytes) + dma_chunk_k * 16;
-  const int dma_lane_off_v = (int)(dma_rr * kv_row_bytes) + dma_chunk_v * 16;
+  const int dma_lane_off_v = (int)(dma_rr * v_row_bytes) + dma_chunk_v * 16;
   // FP8: a unit is 8 raw rows of 128 B, copied as they lie: lane i -> row i / 8, 16-byte piece i % 8
   const int dma_lane_off_raw = (int)((lane >> 3) * kv_row_bytes) + (lane & 7) * 16;
 
   auto lane_row = [&](int key) __attribute__((always_inline)) -> long {   // same, per lane, clamped
     key = min(key, ctx - 1);
     if (MODE == 0) return (long)b * p.S + key;
+    if (PACKED) return key;
     int blk = table[key >> p.block_shift];
     blk = min(max(blk, 0), p.num_blocks - 1);
     return (long)blk * p.block_size + (key & (p.block_size - 1));
@@ -272,7 +329,7 @@ void prefill_async_kernel(PrefillParams p) {
   // copies that need them.  K and V units of a wave share their rows, hence UPW/2 entries.
   int blk_pf[UPW / 2];
   auto prefetch_table = [&](int kt) __attribute__((always_inline)) {
-    if (MODE == 0) return;
+    if (MODE != 1) return;
 #pragma unroll
     for (int i = 0; i < UPW / 2; ++i) {
       const int r0 = FP8 ? 8 * wave : 4 * ((wave + NW * i) & (UK - 1));
@@ -305,19 +362,23 @@ void prefill_async_kernel(PrefillParams p) {
 #pragma unroll
       for (int j = 0; j < UPW / 2; ++j) {
         const int u = (wave + NW * j) & (UK - 1);
-        uint64_t off;
-        if (MODE == 0) {
+        uint64_t off, off_v;
+        if (PACKED) {
+          off = (uint64_t)(uint32_t)(key0 + 4 * u) * kv_row_bytes_u;
+          off_v = (uint64_t)(uint32_t)(key0 + 4 * u) * (uint32_t)v_row_bytes;
+        } else if (MODE == 0) {
           off = (uint64_t)(uint32_t)(b * p.S + key0 + 4 * u) * kv_row_bytes_u;
         } else {
           const uint32_t blk = (uint32_t)min(max(blk_pf[j], 0), p.num_blocks - 1);
           off = (uint64_t)blk * block_bytes_u + (uint32_t)((key0 + 4 * u) & (p.block_size - 1)) * kv_row_bytes_u;
         }
+        if (!PACKED) off_v = off;
         if (PACK && stream_kv) {
           dma16_uniform_stream(kbase + off, dma_lane_off_k, sbase + u * 1024);
-          dma16_uniform_stream(vbase + off, dma_lane_off_v, sbase + TILE_B + u * 1024);
+          dma16_uniform_stream(vbase + off_v, dma_lane_off_v, sbase + TILE_B + u * 1024);
         } else {
           dma16_uniform(kbase + off, dma_lane_off_k, sbase + u * 1024);
-          dma16_uniform(vbase + off, dma_lane_off_v, sbase + TILE_B + u * 1024);
+          dma16_uniform(vbase + off_v, dma_lane_off_v, sbase + TILE_B + u * 1024);
         }
       }
     } else {                                      // last tile of a context: rows past it re-read its last row
@@ -325,7 +386,7 @@ void prefill_async_kernel(PrefillParams p) {
       for (int j = 0; j < UPW; ++j) {
         const bool is_k = j < UPW / 2;
         const int u = (wave + NW * j) & (UK - 1);
-        const char* src = (is_k ? kbase : vbase) + lane_row(key0 + 4 * u + dma_rr) * kv_row_bytes + (is_k ? dma_chunk_k : dma_chunk_v) * 16;
+        const char* src = (is_k ? kbase : vbase) + lane_row(key0 + 4 * u + dma_rr) * (is_k ? kv_row_bytes : v_row_bytes) + (is_k ? dma_chunk_k : dma_chunk_v) * 16;
         if (PACK && stream_kv) dma16_lane_stream(src, sbase + (is_k ? 0 : TILE_B) + u * 1024);
         else dma16_lane(src, sbase + (is_k ? 0 : TILE_B) + u * 1024);
       }
@@ -677,14 +738,14 @@ void prefill_async_kernel(PrefillParams p) {
   prefetch_next();
 #pragma unroll
   for (int j = 0; j < QH; ++j) {
-    const uint16_t* qp = (const uint16_t*)p.q + ((long)b * p.T + qrow) * q_row_stride + (long)(hq_l + j) * DH;
+    const uint16_t* qp = (const uint16_t*)p.q + token_row(qrow) * (PACKED ? p.q_stride : q_row_stride) + (long)(hq_l + j) * DH;
     uint4 qraw[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qraw[s] = make_uint4(0, 0, 0, 0);
       if (qvalid) qraw[s] = *(const uint4*)(qp + 16 * s + 8 * h);
     }
-    if (!SPARSE && p.qt.cos) {
+    if (!SPARSE && !PACKED && p.qt.cos) {
       // norm and rotation of the row on the way in; every lane takes part (the row's other
       // half sits in lane ^ 32), rows past the query length carry zeros
       float x[KS][8];
@@ -911,8 +972,8 @@ void prefill_async_kernel(PrefillParams p) {
       const int r = ORI * j + lane / OCH, ch = lane % OCH;
       const uint2 lo = *(const uint2*)(patch + r * OROW_B + 16 * ch), hi = *(const uint2*)(patch + r * OROW_B + 16 * ch + 8);
       const int tok = row_token(wave * 32 + r);
-      if (tok < p.T && !idle_half)
-        store_stream(out + ((long)b * p.T + tok) * q_row_stride + (long)(row_head(wave * 32 + r) + hj) * DH + 8 * ch,
+      if (tok < seg && !idle_half)
+        store_stream(out + token_row(tok) * q_row_stride + (long)(row_head(wave * 32 + r) + hj) * DH + 8 * ch,
                      make_uint4(lo.x, lo.y, hi.x, hi.y));
     }
   }
@@ -950,6 +1011,48 @@ __global__ __launch_bounds__(256) void prefill_split_reduce_kernel(PrefillParams
   *(uint2*)dst = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
+// The same for packed rows; rows between or behind the sequences stay as they are, rows that see no key become zeros.
+__global__ __launch_bounds__(256) void prefill_packed_reduce_kernel(PrefillParams p) {
+  const long item = (long)blockIdx.x * 256 + threadIdx.x;
+  const int D = p.D;
+  const long row = item / (D / 4);
+  const int q4 = (int)(item % (D / 4));
+  if (row >= (long)p.total_q * p.Hq) return;
+  const int hq = (int)(row % p.Hq);
+  const int at = (int)(row / p.Hq);
+  int lo = 0, hi = p.B;                       // the last sequence that does not begin behind the row
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (min(max(p.cu_q[mid], 0), p.total_q) <= at) lo = mid;
+    else hi = mid;
+  }
+  const int q_first = min(max(p.cu_q[lo], 0), p.total_q), seg = min(max(p.cu_q[lo + 1], 0), p.total_q) - q_first;
+  const int t = at - q_first;
+  if (t < 0 || t >= seg) return;
+  const int seg_k = max(min(max(p.cu_k[lo + 1], 0), p.total_k) - min(max(p.cu_k[lo], 0), p.total_k), 0);
+  const int tq = p.query_lens ? min(max(p.query_lens[lo], 0), seg) : seg;
+  const int ctx = p.seq_lens ? min(max(p.seq_lens[lo], 0), seg_k) : seg_k;
+  uint16_t* dst = (uint16_t*)p.out + row * D + 4 * q4;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (t < tq && ctx - tq + t >= 0) {
+    for (int c = 0; c < p.splits; ++c) {
+      const float2 ml = *(const float2*)(p.ws_ml + (row * p.splits + c) * 2);
+      if (ml.y == 0.f) continue;                 // a share in which the row saw no key (its O may be unwritten)
+      const float4 o = *(const float4*)(p.ws_o + (row * p.splits + c) * D + 4 * q4);
+      const float m_new = fmaxf(m, ml.x);
+      const float a = exp2f(m - m_new), w = exp2f(ml.x - m_new);
+      l = l * a + ml.y * w;
+      acc.x = acc.x * a + o.x * w; acc.y = acc.y * a + o.y * w;
+      acc.z = acc.z * a + o.z * w; acc.w = acc.w * a + o.w * w;
+      m = m_new;
+    }
+    if (p.sinks && l > 0.f) l += exp2f(p.sinks[hq] * kLog2e - m);
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  *(uint2*)dst = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+}
+
 template <bool SPARSE, int MODE, int NW, int TT = 2, bool WIN = false, bool PACK = false, bool SPLIT = false, bool FP8 = false, int DH = HD, int QH = 1>
 hipError_t launch_typed(const PrefillParams& p, hipStream_t s) {
   constexpr int lds = (SPARSE && NW == 8 ? 5 : NW == 8 ? 4 : 2) * 2 * 32 * TT * ROW_B;
@@ -965,12 +1068,19 @@ hipError_t launch_typed(const PrefillParams& p, hipStream_t s) {
   const long per_group = PACK ? ((long)p.T * n_rep + 32 * NW - 1) / (32 * NW)
                               : (long)((p.T + TOKW - 1) / TOKW) * (n_rep / QH);
   const long groups = (long)p.B * (DH == 64 ? (p.Hkv + 1) / 2 : p.Hkv);
-  const long total = 8 * ((groups + 7) / 8) * per_group * (SPLIT ? p.splits : 1);
+  long total = 8 * ((groups + 7) / 8) * per_group * (SPLIT ? p.splits : 1);
+  if (MODE == 2) {       // the kernel's own numbering of (kv head, query tile, q head)
+    const int kvg = DH == 64 ? (p.Hkv + 1) / 2 : p.Hkv, units = n_rep / QH;
+    const long per_head = (long)p.slots * (PACK ? 1 : DH == 64 && p.Hkv == 1 ? (units + 1) / 2 : units);
+    const long items = kvg % 8 == 0 ? kvg / 8 * per_head : 8 % kvg == 0 ? (per_head * kvg + 7) / 8 : (per_head * kvg + 7) / 8;
+    total = 8 * items * (SPLIT ? p.splits : 1);
+  }
   if (total > 0x7fffffffL) return hipErrorInvalidValue;
   hipLaunchKernelGGL((prefill_async_kernel<SPARSE, MODE, NW, TT, WIN, PACK, SPLIT, FP8, DH, QH>), dim3((unsigned)total), dim3(NW * 64), lds, s, p);
   if (SPLIT) {
-    const long items = (long)p.B * p.T * p.Hq * (DH / 4);
-    hipLaunchKernelGGL(prefill_split_reduce_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p);
+    const long items = (MODE == 2 ? (long)p.total_q : (long)p.B * p.T) * p.Hq * (DH / 4);
+    if (MODE == 2) hipLaunchKernelGGL(prefill_packed_reduce_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(prefill_split_reduce_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p);
   }
   return hipGetLastError();
 }
@@ -1111,6 +1221,43 @@ hipError_t launch_prefill_async(const PrefillParams& p, int waves, hipStream_t s
   }
   if (sparse) return launch_typed<true, 0, 4>(p, s);
   return paged ? launch_typed<false, 1, 4>(p, s) : launch_typed<false, 0, 4>(p, s);
+}
+
+// ---- packed form ---------------------------------------------------------------------------------------------
+// 128 packed rows of a kv group (its q heads ride along as rows of one tile), or 256 tokens of one q head
+static bool packed_takes_groups(const PrefillParams& p) {
+  return p.D == HD && p.impl != 8 && (p.impl == 5 || true);
+}
+static int packed_tile_shift(const PrefillParams& p) { return p.D == 64 || packed_takes_groups(p) ? 7 : 8; }
+static int packed_slots(const PrefillParams& p) {
+  const int mult = packed_takes_groups(p) ? p.Hq / p.Hkv : 1;
+  return (int)(((long)mult * p.total_q) >> packed_tile_shift(p)) + p.B;
+}
+
+int prefill_packed_splits(const PrefillParams& p, int num_cus) {
+  (void)p; (void)num_cus;
+  return 1;
+}
+
+hipError_t launch_prefill_packed(const PrefillParams& p0, hipStream_t s) {
+  PrefillParams p = p0;
+  p.slots = packed_slots(p);
+  const bool split = p.splits > 1;
+  if (split && (!p.ws_o || !p.ws_ml)) return hipErrorInvalidValue;
+  if (p.D == 64) {       // (window 0 included: see launch_prefill_async)
+    if (d64_heads_per_wave(p) == 2)
+      return split ? launch_typed<false, 2, 8, 2, true, false, true, false, 64, 2>(p, s)
+                   : launch_typed<false, 2, 8, 2, true, false, false, false, 64, 2>(p, s);
+    return split ? launch_typed<false, 2, 8, 2, true, false, true, false, 64>(p, s)
+                 : launch_typed<false, 2, 8, 2, true, false, false, false, 64>(p, s);
+  }
+  if (p.D != HD) return hipErrorInvalidValue;
+  if (packed_takes_groups(p)) {
+    if (p.window > 0) return split ? launch_typed<false, 2, 4, 2, true, true, true>(p, s) : launch_typed<false, 2, 4, 2, true, true>(p, s);
+    return split ? launch_typed<false, 2, 4, 2, false, true, true>(p, s) : launch_typed<false, 2, 4, 2, false, true>(p, s);
+  }
+  if (p.window > 0) return split ? launch_typed<false, 2, 8, 2, true, false, true>(p, s) : launch_typed<false, 2, 8, 2, true>(p, s);
+  return split ? launch_typed<false, 2, 8, 2, false, false, true>(p, s) : launch_typed<false, 2, 8>(p, s);
 }
 
 }  // namespace pa

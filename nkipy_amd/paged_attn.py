@@ -514,6 +514,87 @@ def blocksparse_prefill(q, k, v, scale, *, block=64, local_blocks=4, vert_stride
     return out
 
 
+_packed_need = {}           # shape key -> scratch bytes of packed_prefill (a pure function of the shape)
+
+
+def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=None, seq_lens=None, max_seq_len=None,
+                   sinks=None, sliding_window=None, out=None, workspace=None):
+    """Causal attention over whole prompts of different lengths, packed row behind row, with dense K and V.
+
+    q [Nq, Hq, D], k / v [Nk, Hkv, D] bfloat16 (head_dim 64 or 128); sequence i owns rows cu_seqlens[i] ..
+    cu_seqlens[i + 1] - 1 of q and of the result, and rows cu_seqlens_k[i] .. of k and v (default: the same rows).
+    The attention of examples/models/qwen3/kernels/attention.py:112-144 for each sequence; with more keys than queries
+    the queries are the last ones (gpt_oss/kernels/attention.py:85,127-135): query t of n sees keys j <= c - n + t of c.
+    This is the prompt's own attention, before or beside the cache write (`kv_write` with the same cu_seqlens), and,
+    with keys that `read_kv` has read back, that of the next chunk of a prompt whose first part is cached.
+
+    q, k and v may be slices of a wider tensor (the heads of a token adjacent, any token stride that is a multiple of 8
+    elements): the output of a fused projection as it is.  cu_seqlens int32 [num_seqs + 1].
+    query_lens / seq_lens int32 [num_seqs]: of a sequence's rows only the first query_lens[i] are queries and the first
+    seq_lens[i] keys (rows laid out with room to spare); the other query rows are padding, zero in the result, and the
+    other keys are never read.  A query that sees no key gets zeros; rows that belong to no sequence are left as they
+    are (whatever the memory held in a result allocated here).
+    K and V rows are expected to be finite: a V row with an infinity or a NaN reaches the rows of up to 255 queries
+    in front of it as well (their weight for it is 0, and 0 x inf is not).
+    max_seq_len: host-known upper bound of a sequence's keys; sizes the split of calls with few queries over many keys
+    (default Nk).  sinks [Hq] / sliding_window as in `decode`, the window counted back from each query.
+    """
+    lib = _lib.load()
+    qs, ks, vs = _token_rows("q", q), _token_rows("k", k), _token_rows("v", v)
+    Nq, Hq, D = q.shape
+    Nk, Hkv = k.shape[:2]
+    _check(k.shape[2] == D and v.shape == k.shape, "k and v must be [Nk, Hkv, D] with q's D")
+    _check(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"Hq={Hq} is not a multiple of Hkv={Hkv}")
+    _check(D in (64, 128), f"head_dim {D} must be 64 or 128")
+    _need_device("cu_seqlens", cu_seqlens)
+    _check(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "cu_seqlens must be int32 [num_seqs + 1]")
+    S = cu_seqlens.shape[0] - 1
+    _check_cu("cu_seqlens", cu_seqlens, S)
+    if cu_seqlens_k is None:
+        cu_seqlens_k = cu_seqlens
+        _check(Nk == Nq, f"k has {Nk} rows, q {Nq}: give cu_seqlens_k")
+    else:
+        _check_cu("cu_seqlens_k", cu_seqlens_k, S)
+    for n, t in (("query_lens", query_lens), ("seq_lens", seq_lens)):
+        if t is not None:
+            _need_device(n, t)
+            _check(t.shape == (S,) and t.dtype == torch.int32, f"{n} must be int32 [num_seqs]")
+    _check(max_seq_len is None or int(max_seq_len) > 0, f"max_seq_len {max_seq_len} must be positive")
+    bound = Nk if max_seq_len is None else min(int(max_seq_len), Nk)
+    sinks, win = _check_variant(sinks, sliding_window, Hq, q)
+    if out is None:
+        out = torch.empty((Nq, Hq, D), dtype=torch.bfloat16, device=q.device)
+    else:
+        _need_device("out", out)
+        _check(tuple(out.shape) == (Nq, Hq, D) and out.dtype == torch.bfloat16, f"out must be bfloat16 {(Nq, Hq, D)}")
+    _same_device(q, k=k, v=v, cu_seqlens=cu_seqlens, cu_seqlens_k=cu_seqlens_k, query_lens=query_lens, seq_lens=seq_lens, out=out)
+    with _on(q.device):
+        stream = _stream_ptr(q.device)
+        key = (S, Nq, Nk, Hq, Hkv, D, bound)
+        need = _packed_need.get(key)
+        if need is None:
+            if len(_packed_need) >= 4096:
+                _packed_need.clear()
+            need = _packed_need[key] = int(lib.pa_packed_prefill_workspace_bytes(*key))
+        if workspace is None:
+            workspace = _workspace(q.device, need, stream) if need else None
+        else:
+            _need_device("workspace", workspace)
+            _same_device(q, workspace=workspace)
+            _check(workspace.numel() * workspace.element_size() >= need, f"workspace needs {need} bytes")
+        ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+        rc = lib.pa_packed_prefill(_ptr(q), _ptr(k), _ptr(v), qs, ks, vs, _ptr(cu_seqlens), _ptr(cu_seqlens_k), _ptr(query_lens),
+                                   _ptr(seq_lens), _ptr(out), _ptr(workspace), ws_bytes, S, Nq, Nk, Hq, Hkv, D, bound,
+                                   float(scale), BF16, _ptr(sinks), win, stream)
+    _raise_on(rc, "pa_packed_prefill")
+    return out
+
+
+def packed_prefill_workspace_bytes(num_seqs: int, total_q: int, total_k: int, Hq: int, Hkv: int, D: int, max_seq_len: int) -> int:
+    """Scratch bytes `packed_prefill` would use (0 for calls that take none)."""
+    return int(_lib.load().pa_packed_prefill_workspace_bytes(num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len))
+
+
 def gather_kv(cache, block_tables, seq_lens, max_seq_len=None):
     """Materialise the block-table gather: [B, max_seq_len, Hkv, D], zero past seq_lens[b]."""
     lib = _lib.load()

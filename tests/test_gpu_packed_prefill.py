@@ -1,0 +1,204 @@
+"""Packed prompt attention on the GPU against float64, element by element within what the roundings allow."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_attention_oracle as O
+from tests.int8_kv_lib import assert_within, attention64, attention_tolerance, bf16, dev
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def pa():
+    import nkipy_amd
+    from nkipy_amd import _lib
+    _lib.load()
+    return nkipy_amd
+
+
+@pytest.fixture
+def debug_switch():
+    from nkipy_amd import _lib
+    lib = _lib.load()
+    yield lambda key, value: lib.pa_debug_set(key, value)
+    lib.pa_debug_set(3, 0)
+    lib.pa_debug_set(6, 1)
+
+
+def _starts(n):
+    return np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+
+
+def _want(q, k, v, cu_q, cu_k, scale, window, sinks, qlens=None, klens=None):
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    for i in range(len(cu_q) - 1):
+        n = cu_q[i + 1] - cu_q[i] if qlens is None else min(qlens[i], cu_q[i + 1] - cu_q[i])
+        c = cu_k[i + 1] - cu_k[i] if klens is None else min(klens[i], cu_k[i + 1] - cu_k[i])
+        rows = slice(cu_q[i], cu_q[i] + n)
+        o, mag, reach = attention64(q[rows].astype(np.float64), k[cu_k[i]:cu_k[i] + c].astype(np.float64),
+                                    v[cu_k[i]:cu_k[i] + c].astype(np.float64), scale, c - n, window or 0, sinks)
+        out[rows], tol[rows] = o, attention_tolerance(o, mag, reach, q.shape[2], q_rounded=True)
+    return out, tol
+
+
+def _run(pa, rng, qn, Hq, Hkv, D, kn=None, window=None, with_sinks=False, strided=False, tail=0, **kw):
+    cu_q = _starts(qn)
+    cu_k = cu_q if kn is None else _starts(kn)
+    nq, nk = int(cu_q[-1]) + tail, int(cu_k[-1]) + tail
+    q, k, v = (O.round_to_bf16(rng.standard_normal((n, h, D)).astype(np.float32)) for n, h in ((nq, Hq), (nk, Hkv), (nk, Hkv)))
+    scale = 1.0 / np.sqrt(D)
+    sinks = rng.standard_normal(Hq).astype(np.float32) if with_sinks else None
+    if strided:
+        wide = torch.full((nq, Hq + 2 * Hkv + 1, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+        dq, dk, dv = wide[:, :Hq], wide[:, Hq:Hq + Hkv], wide[:, Hq + Hkv + 1:]
+        dq.copy_(bf16(q)), dk.copy_(bf16(k)), dv.copy_(bf16(v))
+    else:
+        dq, dk, dv = bf16(q), bf16(k), bf16(v)
+    if tail:
+        dk[-tail:] = float("nan")
+        dv[-tail:] = float("nan")
+    out = torch.full((nq, Hq, D), 3.0, dtype=torch.bfloat16, device="cuda")
+    got = pa.packed_prefill(dq, dk, dv, dev(cu_q), scale, cu_seqlens_k=None if kn is None else dev(cu_k), sliding_window=window,
+                            sinks=None if sinks is None else dev(sinks), out=out, **kw)
+    want, tol = _want(q, k, v, cu_q, cu_k, scale, window, sinks)
+    if tail:
+        assert (got[-tail:] == 3.0).all()
+        got, want, tol = got[:-tail], want[:-tail], tol[:-tail]
+    assert_within(got, want, tol)
+    return dq, dk, dv, got
+
+
+HEADS = [(8, 2, 128), (4, 4, 128), (6, 1, 128), (5, 5, 128), (12, 2, 64), (8, 4, 64), (6, 3, 64), (5, 1, 64), (8, 1, 64), (2, 2, 64),
+         (1, 1, 64), (20, 10, 128)]
+
+
+@pytest.mark.parametrize("impl", [0, 8])
+@pytest.mark.parametrize("Hq,Hkv,D", HEADS)
+def test_ragged_prompts(pa, rng, debug_switch, Hq, Hkv, D, impl):
+    debug_switch(3, impl)
+    _run(pa, rng, [1, 64, 0, 63, 129, 300, 2, 65, 33, 0], Hq, Hkv, D, tail=5)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (64, 8, 64), (16, 2, 128), (16, 16, 64)])
+def test_strided_rows(pa, rng, Hq, Hkv, D):
+    _run(pa, rng, [100, 1, 200, 17], Hq, Hkv, D, strided=True)
+
+
+@pytest.mark.parametrize("impl", [0, 8])
+@pytest.mark.parametrize("split", [1, 0, 2, 5, 16])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (8, 2, 64), (3, 1, 64), (3, 3, 128)])
+def test_more_keys_than_queries_and_fewer(pa, rng, debug_switch, Hq, Hkv, D, split, impl):
+    """Cached prefixes, sequences with fewer keys than queries (their first rows see nothing), and with none at all."""
+    debug_switch(3, impl)
+    debug_switch(6, split)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    _run(pa, rng, [40, 1, 130, 3, 70, 20], Hq, Hkv, D, kn=[400, 777, 130, 0, 5, 65], tail=3, workspace=ws)
+
+
+@pytest.mark.parametrize("split", [1, 3])
+@pytest.mark.parametrize("window", [1, 30, 64, 200, 5000])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (8, 4, 64), (6, 3, 64)])
+def test_window_and_sinks(pa, rng, debug_switch, Hq, Hkv, D, window, split):
+    debug_switch(6, split)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    _run(pa, rng, [150, 1, 300, 31], Hq, Hkv, D, kn=[150, 260, 700, 31], window=window, with_sinks=True, workspace=ws)
+
+
+@pytest.mark.parametrize("split", [1, 2])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (8, 2, 64)])
+def test_rows_with_room_to_spare(pa, rng, debug_switch, Hq, Hkv, D, split):
+    """query_lens / seq_lens: padding query rows are zero, key rows past the length (NaN here) are never used, gaps too."""
+    debug_switch(6, split)
+    cu_q, cu_k = _starts([64, 64, 64, 64, 200]), _starts([300, 300, 300, 300, 300])
+    qlens, klens = [64, 1, 0, 30, 150], [300, 17, 200, 20, 260]
+    q = O.round_to_bf16(rng.standard_normal((int(cu_q[-1]), Hq, D)).astype(np.float32))
+    k, v = (O.round_to_bf16(rng.standard_normal((int(cu_k[-1]), Hkv, D)).astype(np.float32)) for _ in range(2))
+    dk, dv = bf16(k), bf16(v)
+    for i, c in enumerate(klens):
+        dk[cu_k[i] + c:cu_k[i + 1]] = float("nan")
+        dv[cu_k[i] + c:cu_k[i + 1]] = float("inf")
+    i32 = lambda x: dev(np.asarray(x, np.int32))               # noqa: E731
+    got = pa.packed_prefill(bf16(q), dk, dv, dev(cu_q), 0.1, cu_seqlens_k=dev(cu_k), query_lens=i32(qlens), seq_lens=i32(klens),
+                            workspace=torch.empty(64 << 20, dtype=torch.uint8, device="cuda"))
+    want, tol = _want(q, k, v, cu_q, cu_k, 0.1, None, None, qlens, klens)
+    assert_within(got, want, tol)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (16, 4, 64)])
+def test_against_the_paged_kernel(pa, rng, Hq, Hkv, D):
+    """The same prompt through a paged bfloat16 pool, written packed."""
+    n, bs = 700, 32
+    q, k, v = (bf16(rng.standard_normal((n, h, D))) for h in (Hq, Hkv, Hkv))
+    cu = dev(np.asarray([0, n], np.int32))
+    got = pa.packed_prefill(q, k, v, cu, 0.1)
+    blocks = (n + bs - 1) // bs
+    kc, vc = (torch.zeros((blocks, bs, Hkv, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    tables = dev(rng.permutation(blocks).astype(np.int32)[None])
+    ln = dev(np.asarray([n], np.int32))
+    pa.kv_write(k, v, kc, vc, tables, ln, ln, cu_seqlens=cu)
+    ref = pa.prefill(q[None], kc, vc, tables, ln, ln, 0.1)[0]
+    assert (got.float() - ref.float()).abs().max() <= 2e-2
+    k2, v2 = pa.read_kv(kc, vc, tables, ln, cu, n)
+    assert torch.equal(k2, k) and torch.equal(v2, v)
+
+
+def test_large_scores_move_the_reference(pa, rng):
+    """Scores that grow along the keys by far more than float32's exponent range allows for a fixed reference."""
+    n, D = 400, 128
+    q, k, v = (O.round_to_bf16(rng.standard_normal((n, 2, D)).astype(np.float32)) for _ in range(3))
+    q[:] = 1.0
+    k *= 0.05
+    k += O.round_to_bf16(np.linspace(-40, 60, n).astype(np.float32))[:, None, None]
+    k = O.round_to_bf16(k)
+    got = pa.packed_prefill(bf16(q), bf16(k), bf16(v), dev(np.asarray([0, n], np.int32)), 0.125)
+    want, tol = _want(q, k, v, [0, n], [0, n], 0.125, None, None)
+    assert_within(got, want, tol)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_other_scales(pa, rng, scale):
+    n, D = 150, 64
+    q, k, v = (O.round_to_bf16(rng.standard_normal((n, 2, D)).astype(np.float32)) for _ in range(3))
+    got = pa.packed_prefill(bf16(q), bf16(k), bf16(v), dev(np.asarray([0, n], np.int32)), scale)
+    want, tol = _want(q, k, v, [0, n], [0, n], scale, None, None)
+    assert_within(got, want, tol)
+
+
+def test_boundaries_that_lie(pa, rng):
+    """Boundaries outside the tensors count as their ends: nothing outside is read or written."""
+    n, D = 130, 128
+    q, k, v = (bf16(rng.standard_normal((n, 2, D))) for _ in range(3))
+    for cu in ([0, 1 << 30], [-5, 2 ** 31 - 1], [50, 10], [0, 100, 20, 130], [-2 ** 31, 2 ** 31 - 1], [200, 300]):
+        out = pa.packed_prefill(q, k, v, dev(np.asarray(cu, np.int32)), 0.1, out=torch.zeros_like(q))
+        assert torch.isfinite(out).all()
+    full = pa.packed_prefill(q, k, v, dev(np.asarray([-5, 2 ** 31 - 1], np.int32)), 0.1)
+    assert torch.equal(full, pa.packed_prefill(q, k, v, dev(np.asarray([0, n], np.int32)), 0.1))
+
+
+def test_graph_replays_with_other_lengths(pa, rng):
+    D, Hq, Hkv, n = 128, 8, 2, 512
+    q, k, v = (torch.zeros((n, h, D), dtype=torch.bfloat16, device="cuda") for h in (Hq, Hkv, Hkv))
+    cu = dev(_starts([200, 312]))
+    run = lambda: pa.packed_prefill(q, k, v, cu, 0.1)          # noqa: E731
+    for x in (q, k, v):
+        x.copy_(bf16(rng.standard_normal(x.shape)))
+    run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    for lens in ([200, 312], [1, 511], [512, 0], [256, 100]):
+        cu.copy_(dev(_starts(lens)))
+        for x in (q, k, v):
+            x.copy_(bf16(rng.standard_normal(x.shape)))
+        g.replay()
+        torch.cuda.synchronize()
+        a = out[:sum(lens)].clone()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            b = run()
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        assert torch.equal(a, b[:sum(lens)])
