@@ -91,6 +91,51 @@ template <> struct Store<uint16_t> {
   }
 };
 
+// Inclusive prefix sum over the 64 lanes of a wave on DPP adds: shifts by 1, 2, 4 and 8 inside each row of 16 lanes
+// (a lane without a source adds 0), then lane 15 of rows 0 and 2 into rows 1 and 3, then lane 31 into rows 2 and 3.
+__device__ __forceinline__ int wave_inclusive_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111 /* row_shr:1 */, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112 /* row_shr:2 */, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114 /* row_shr:4 */, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118 /* row_shr:8 */, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142 /* row_bcast:15 */, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143 /* row_bcast:31 */, 0xc, 0xf, false);
+  return x;
+}
+// the same steps for the maximum of non-negative numbers, which every lane gets
+__device__ __forceinline__ int wave_max_nonneg(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// ---- division by a number the host knows -----------------------------------------------
+// floor(x / d) of any 32-bit x as a high product, an add and two shifts (the round-up method: with s = ceil(log2 d) and
+// m = floor(2^32 (2^s - d) / d) + 1, the quotient is (t + ((x - t) >> min(s, 1))) >> max(s - 1, 0), t = floor(m x / 2^32)).
+// An integer division by a run-time number is some forty instructions on this target, and a workgroup of a short
+// sequence would spend as long dividing as attending.
+struct FastDiv {
+  uint32_t m, d;
+  int s1, s2;
+  void set(uint32_t n) {
+    d = n;
+    int s = 0;
+    while ((1ull << s) < n) ++s;
+    m = (uint32_t)((((1ull << 32) * ((1ull << s) - n)) / n) + 1);
+    s1 = s < 1 ? s : 1;
+    s2 = s > 1 ? s - 1 : 0;
+  }
+  __device__ __forceinline__ int quot(int x) const {
+    const uint32_t t = __umulhi(m, (uint32_t)x);
+    return (int)((t + (((uint32_t)x - t) >> s1)) >> s2);
+  }
+  __device__ __forceinline__ int rem(int x) const { return x - quot(x) * (int)d; }
+};
+
 // ---- packed rows -------------------------------------------------------------------
 // Sequence i of n owns rows [cu[i], cu[i + 1]) of a packed tensor of `total` rows.  Work is dealt in tiles of 2^shift
 // units of one sequence, a row being `mult` units; tile t of sequence i has the number floor(mult cu[i] / 2^shift) + i + t,
@@ -303,6 +348,10 @@ struct PrefillParams {
   int total_q, total_k;     // rows of q and of k / v
   long q_stride, k_stride, v_stride;    // elements from one token to the next
   int slots;                // query tiles are numbered 0 .. slots - 1 (packed_find)
+  int n_rep;                // Hq / Hkv
+  int kvg, hpg;             // kv heads (pairs of them at head dim 64); workgroups per query tile and such group
+  int deal;                 // how kv heads are dealt over the XCDs: 0 each XCD its own, else so many XCDs share one, -1 in turn
+  FastDiv by_rep, by_hpg, by_kvg, by_head, by_splits;   // by_head: slots x hpg
   int num_cus;              // CUs of the device the call runs on (0: unknown, taken as 256); steers the workgroup shape
   int len_bound;            // the caller's bound on the sequence lengths (0: none); steers the workgroup shape as well
 };

@@ -172,6 +172,7 @@ struct DecodeWave {
   uint4* qlds;               // LEAN: this wave's [R][KSTEPS][64] fragment store in LDS
   int qlane;                 // LEAN: lane index into it, re-made opaque per tile so the reads stay in the loop
   bf16x8_t pf[R];            // P^T fragments of the current tile
+  bf16x8_t pl[I8 ? R : 1];   // int8: what their rounding left over
   f32x4_t oacc[R][VEC];
   float m_run[R], l_run[R];
   // NEWROW: chunk 4 s + g of the new K row (the lane's operand piece in k-step s, as transformed), the lane's
@@ -637,8 +638,18 @@ struct DecodeWave {
 #pragma unroll
         for (int i = 0; i < 8; ++i) pr[i] = sv[i] == -INFINITY ? 0.f : pr[i] * vt.vsc[i % (I8 ? 8 : 2)];
       }
-      pf[rg] = as_bf16x8(pack_bf16x2(pr[0], pr[1]), pack_bf16x2(pr[2], pr[3]),
-                         pack_bf16x2(pr[4], pr[5]), pack_bf16x2(pr[6], pr[7]));
+      const uint32_t pw[4] = {pack_bf16x2(pr[0], pr[1]), pack_bf16x2(pr[2], pr[3]), pack_bf16x2(pr[4], pr[5]), pack_bf16x2(pr[6], pr[7])};
+      pf[rg] = as_bf16x8(pw[0], pw[1], pw[2], pw[3]);
+      if (I8) {
+        // The codes are exact in bf16, so the one rounding on the way is that of the probabilities (with their value's
+        // scale): 2^-8 each, as much again as the rounding of the result.  A second operand takes what it left
+        // over (another 8 bits); this kernel waits for memory, not for the matrix pipeline.
+        uint32_t lw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          lw[i] = pack_bf16x2(pr[2 * i] - __uint_as_float(pw[i] << 16), pr[2 * i + 1] - __uint_as_float(pw[i] & 0xffff0000u));
+        pl[I8 ? rg : 0] = as_bf16x8(lw[0], lw[1], lw[2], lw[3]);
+      }
     }
   }
 
@@ -655,9 +666,11 @@ struct DecodeWave {
           for (int jp = 0; jp < 4; ++jp)
             w[jp] = pack_hi16(i8_to_float<decltype(eb)::value>(tl.v[2 * jp][dw]), i8_to_float<decltype(eb)::value>(tl.v[2 * jp + 1][dw]));
 #pragma unroll
-          for (int rg = 0; rg < R; ++rg)
-            oacc[rg][4 * dw + decltype(eb)::value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                as_bf16x8(w[0], w[1], w[2], w[3]), pf[rg], oacc[rg][4 * dw + decltype(eb)::value], 0, 0, 0);
+          for (int rg = 0; rg < R; ++rg) {
+            f32x4_t& o = oacc[rg][4 * dw + decltype(eb)::value];
+            o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(w[0], w[1], w[2], w[3]), pf[rg], o, 0, 0, 0);
+            o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(w[0], w[1], w[2], w[3]), pl[I8 ? rg : 0], o, 0, 0, 0);
+          }
         };
         column(std::integral_constant<int, 0>{});
         column(std::integral_constant<int, 1>{});
@@ -1126,17 +1139,6 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 1 : 2) void decode_mfma_kernel(De
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int tiles_of(int ctx) { return (ctx + 31) >> 5; }
 
-// Inclusive prefix sum over the 64 lanes of a wave on DPP adds: shifts by 1, 2, 4 and 8 inside each row of 16 lanes
-// (a lane without a source adds 0), then lane 15 of rows 0 and 2 into rows 1 and 3, then lane 31 into rows 2 and 3.
-__device__ __forceinline__ int wave_inclusive_sum(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111 /* row_shr:1 */, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112 /* row_shr:2 */, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114 /* row_shr:4 */, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118 /* row_shr:8 */, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142 /* row_bcast:15 */, 0xa, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143 /* row_bcast:31 */, 0xc, 0xf, false);
-  return x;
-}
 // Tiles of sequence b that the schedule streams: all of them, or those the window reaches
 __device__ __forceinline__ int span_tiles(const DecodeParams& p, int b) {
   const int ctx = clamp_ctx(p, b);

@@ -31,6 +31,7 @@
 //
 // Masking follows examples/models/gpt_oss/kernels/attention.py:85,127-135: query
 // i of a chunk that starts at `prefix` sees keys j <= prefix + i.
+#include <algorithm>
 #include <atomic>
 
 #include "pa_common.h"
@@ -92,6 +93,100 @@ __device__ __forceinline__ void dma16_lane_stream(const char* addr, uint32_t lds
 // waited for in order with the copies above.
 typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
 
+// Which query tile of which sequence a workgroup of the packed form takes.
+struct PackedTile {
+  int b, tile, tiles;        // sequence, its query tile (negative: nothing for this workgroup), its number of tiles
+  int q_first, seg;          // its first row in q / out and their number
+  int k_first, seg_k;        // ... and in k / v
+  int tq, ctx;               // queries and keys among them
+};
+// Number x of the query tiles of all sequences in the order of the keys they reach, most first.  A causal tile's work
+// grows with its place, sequences differ in length, and a tile that walks a hundred key tiles started last would be
+// the launch's tail.  With n <= 512 sequences their tile counts fit the wave's registers: tile t of sequence i has the
+// key K_i + t (K_i: its cached prefix in tiles), the number of tiles with a key of at least L is sum_i min(T_i, max(0,
+// K_i + T_i - L)), and L is found bit by bit with one wave sum each; among the sequences that have a tile of that very
+// key the order is theirs.  No pass of its own, no workspace, about 1.3 us per
+// workgroup with its loads, which the other workgroup of the CU covers.   More sequences take
+// their own order (packed_find).  All lanes of all waves run this alike.
+template <int C>       // up to 64 C sequences, C per lane
+__device__ __forceinline__ PackedTile packed_tile_ranked(const PrefillParams& p, int x, int shift, int mult, int lane) {
+  PackedTile r;
+  int T[C], K[C], qf[C], sg[C], kf[C], sk[C], tq[C], cx[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    T[c] = K[c] = qf[c] = sg[c] = kf[c] = sk[c] = tq[c] = cx[c] = 0;
+    const int i = 64 * c + lane;
+    if (64 * c < p.B && i < p.B) {
+      qf[c] = min(max(p.cu_q[i], 0), p.total_q);
+      sg[c] = max(min(max(p.cu_q[i + 1], 0), p.total_q) - qf[c], 0);
+      kf[c] = min(max(p.cu_k[i], 0), p.total_k);
+      sk[c] = max(min(max(p.cu_k[i + 1], 0), p.total_k) - kf[c], 0);
+      tq[c] = p.query_lens ? min(max(p.query_lens[i], 0), sg[c]) : sg[c];
+      cx[c] = p.seq_lens ? min(max(p.seq_lens[i], 0), sk[c]) : sk[c];
+      T[c] = (sg[c] * mult + (1 << shift) - 1) >> shift;
+      K[c] = (int)min((long)max(cx[c] - tq[c], 0) * mult >> shift, 1L << 28);
+    }
+  }
+  auto at_least = [&](int L) __attribute__((always_inline)) {
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (64 * c < p.B) n += min(T[c], max(0, K[c] + T[c] - L));
+    return __builtin_amdgcn_readlane(wave_inclusive_sum(n), 63);
+  };
+  r.tile = -1;
+  r.b = r.tiles = r.q_first = r.seg = r.k_first = r.seg_k = r.tq = r.ctx = 0;
+  if (x >= at_least(0)) return r;
+  int top = 0;
+#pragma unroll
+  for (int c = 0; c < C; ++c) top = max(top, T[c] > 0 ? K[c] + T[c] : 0);
+  top = wave_max_nonneg(top);
+  int L = 0, above = 0;                     // at_least(L) > x always; above = at_least(L + 1) in the end
+  for (int bit = 1 << (31 - __clz(top)); bit; bit >>= 1) {
+    const int n = at_least(L + bit);
+    if (n > x) L += bit;
+    else above = n;
+  }
+  int left = x - above;
+  bool found = false;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (64 * c >= p.B || found) continue;
+    const bool has = K[c] <= L && L < K[c] + T[c];
+    const unsigned long long m = __ballot(has);
+    const int n = __popcll(m);
+    if (left < n) {
+      const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+      const int idx = __ffsll((long long)__ballot(has && below == left)) - 1;
+      auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, idx); };
+      r.b = 64 * c + idx;
+      r.tile = L - of(K[c]);
+      r.tiles = of(T[c]);
+      r.q_first = of(qf[c]); r.seg = of(sg[c]); r.k_first = of(kf[c]); r.seg_k = of(sk[c]); r.tq = of(tq[c]); r.ctx = of(cx[c]);
+      found = true;
+    }
+    left -= n;
+  }
+  return r;
+}
+
+__device__ __forceinline__ PackedTile packed_tile(const PrefillParams& p, int x, int shift, int mult, int lane) {
+  PackedTile r;
+  if (p.B > 512) {
+    r.b = packed_find(as_packed(p.cu_q), p.B, p.total_q, shift, x, &r.tile, mult);
+    r.q_first = packed_row(as_packed(p.cu_q), r.b, p.total_q);
+    r.seg = packed_row(as_packed(p.cu_q), r.b + 1, p.total_q) - r.q_first;
+    r.k_first = packed_row(as_packed(p.cu_k), r.b, p.total_k);
+    r.seg_k = max(packed_row(as_packed(p.cu_k), r.b + 1, p.total_k) - r.k_first, 0);
+    r.tq = min(max(p.query_lens ? p.query_lens[r.b] : r.seg, 0), max(r.seg, 0));
+    r.ctx = min(max(p.seq_lens ? p.seq_lens[r.b] : r.seg_k, 0), r.seg_k);
+    r.tiles = r.seg > 0 ? (r.seg * mult + (1 << shift) - 1) >> shift : 0;
+    r.tile = r.tile >= r.tiles ? -1 : r.tiles - 1 - r.tile;
+    return r;
+  }
+  return p.B <= 64 ? packed_tile_ranked<1>(p, x, shift, mult, lane) : packed_tile_ranked<8>(p, x, shift, mult, lane);
+}
+
 // MODE: 0 = dense K/V [B, S, Hkv, D]; 1 = paged, block size a power of two >= 16; 2 = packed: sequences of different
 // lengths row behind row, dense K/V (p.cu_q, p.cu_k).
 // TT: 32-key sub-tiles per key tile (2: 64-key tiles).
@@ -132,9 +227,15 @@ void prefill_async_kernel(PrefillParams p) {
   // of the waves works for it and the first half only copies (`idle_half`).
   constexpr bool PAIR = DH == 64;
   constexpr bool PACKED = MODE == 2;
-  static_assert(DH == HD || (PAIR && NW == 8 && MODE != 0 && !SPARSE && !PACK), "head dim 64: 8-wave paged or packed form only");
+  static_assert(DH == HD || (PAIR && NW == (PACKED ? 4 : 8) && MODE != 0 && !SPARSE && !PACK), "head dim 64: 8-wave paged form, 4-wave packed form");
   static_assert(!PACKED || (!SPARSE && !FP8), "packed form: plain causal attention over bf16 rows");
   static_assert(QH == 1 || (QH == 2 && PAIR), "two q heads per wave: head dim 64 only");
+  // Packed form: the queries go into the score product as they are, and the scale and the reference are one
+  // fused multiply-add per score, the accumulators starting at zero.  (With the
+  // scale in Q, which rounds every element of it once more, the results of 32 prompts of 17-256 tokens are off by 1.5
+  // times, of 4 096 cached keys by 2.2 times what their own rounding to bf16 costs, root mean square against float64;
+  // this way by 1.4 times, the rounding of the probabilities being the other part.  It costs 4 % on long prompts: 2 of 4 097-8 192 tokens, 869 -> 905 us.)
+  constexpr bool EXACT_Q = PACKED;
   constexpr int KS = DH / 16;                // k-steps of the score product
   constexpr int VC = DH / 32;                // 32-wide d chunks of the output
   constexpr int TOKW = PAIR ? BMW / 2 : BMW; // query tokens per workgroup (plain form)
@@ -160,54 +261,50 @@ void prefill_async_kernel(PrefillParams p) {
   // (consecutive workgroup ids go to consecutive XCDs), and all query tiles and q heads
   // that share one kv head run on one XCD, back to back, heavy tiles first: their K/V
   // stays in that XCD's L2.
-  const int n_rep = p.Hq / p.Hkv;
-  const int nqt = PACK ? (p.T * n_rep + BMW - 1) / BMW : (p.T + TOKW - 1) / TOKW;
-  const int kvg = PAIR ? (p.Hkv + 1) / 2 : p.Hkv;    // K/V row groups: kv heads, or pairs of them
+  const int n_rep = PACKED ? p.n_rep : p.Hq / p.Hkv;
+  const int nqt = PACKED ? 0 : PACK ? (p.T * n_rep + BMW - 1) / BMW : (p.T + TOKW - 1) / TOKW;
+  const int kvg = PACKED ? p.kvg : PAIR ? (p.Hkv + 1) / 2 : p.Hkv;    // K/V row groups: kv heads, or pairs of them
   // Packed form over a single kv head of 64: there is no second head for the other half of a 256-byte row; both halves
   // of the tile hold that head (`solo`), and the two halves of the waves work for different q heads of it.
   const bool solo = PACKED && PAIR && p.Hkv == 1;
   const int units = n_rep / QH;                // q heads (or pairs of them) of a kv head
-  const int hpg = solo ? (units + 1) / 2 : units;    // workgroups (per query tile) that cover the q heads of a kv head
-  const int part = SPLIT ? (int)(blockIdx.x >> 3) % p.splits : 0;      // which share of the key tiles
-  const int slot = SPLIT ? (int)(blockIdx.x >> 3) / p.splits : (int)(blockIdx.x >> 3);
+  const int hpg = PACKED ? p.hpg : units;      // workgroups (per query tile) that cover the q heads of a kv head
+  const int part = !SPLIT ? 0 : PACKED ? p.by_splits.rem(blockIdx.x >> 3) : (int)(blockIdx.x >> 3) % p.splits;      // which share of the key tiles
+  const int slot = !SPLIT ? (int)(blockIdx.x >> 3) : PACKED ? p.by_splits.quot(blockIdx.x >> 3) : (int)(blockIdx.x >> 3) / p.splits;
   const int xcd = blockIdx.x & 7;
   int b, hk, rr_, qt;                          // sequence, kv head (PAIR: pair of them), q head (pair) of the group, query tile
   bool stream_kv;                              // PACK with one row tile per kv head: the only reader of its keys and values
   int seg, q_first, k_first, seg_k;            // packed: rows of the sequence and its first row, in q and in k / v
+  int pk_tq = 0, pk_ctx = 0;                   // ... and the queries and keys among them
   if constexpr (PACKED) {
     // All kv heads have the same work, so they are dealt over the XCDs: with a multiple of eight heads each XCD has its
     // own ones, with one, two or four several XCDs share a head's query tiles, and any other number takes the heads in
     // turn.  The q heads of a tile come next to one another.
     int rest;
-    if (kvg % 8 == 0) {
-      const int per_head = p.slots * (PACK ? 1 : hpg);
-      hk = xcd + 8 * (slot / per_head);
-      rest = slot % per_head;
-    } else if (8 % kvg == 0) {
-      hk = xcd % kvg;
-      rest = slot * (8 / kvg) + xcd / kvg;
+    if (p.deal == 0) {
+      const int turn = p.by_head.quot(slot);
+      hk = xcd + 8 * turn;
+      rest = slot - turn * (int)p.by_head.d;
+    } else if (p.deal > 0) {                   // 8 / kvg XCDs per head: kvg is 1, 2 or 4
+      hk = xcd & (kvg - 1);
+      rest = slot * p.deal + p.by_kvg.quot(xcd);
     } else {
       const int item = slot * 8 + xcd;
-      hk = item % kvg;
-      rest = item / kvg;
+      rest = p.by_kvg.quot(item);
+      hk = item - rest * kvg;
     }
     if (hk >= kvg) return;
-    const int number = PACK ? rest : rest / hpg;
-    rr_ = PACK ? 0 : rest % hpg;
+    const int number = PACK ? rest : p.by_hpg.quot(rest);
+    rr_ = PACK ? 0 : rest - number * hpg;
     if (number >= p.slots) return;
-    constexpr int SHIFT = (TOKW == 256 ? 8 : 7);
-    static_assert(TOKW == 256 || TOKW == 128, "query tiles of 128 or 256 rows");
-    const int mult = PACK ? n_rep : 1;
-    int tile;
-    b = packed_find(as_packed(p.cu_q), p.B, p.total_q, SHIFT, number, &tile, mult);
-    q_first = packed_row(as_packed(p.cu_q), b, p.total_q);
-    seg = packed_row(as_packed(p.cu_q), b + 1, p.total_q) - q_first;
-    k_first = packed_row(as_packed(p.cu_k), b, p.total_k);
-    seg_k = max(packed_row(as_packed(p.cu_k), b + 1, p.total_k) - k_first, 0);
-    const int tiles = (seg * mult + TOKW - 1) >> SHIFT;
-    if (tile < 0 || tile >= tiles) return;
-    qt = tiles - 1 - tile;                     // the tiles with the most keys first
-    stream_kv = PACK && tiles == 1;
+    constexpr int SHIFT = TOKW == 256 ? 8 : TOKW == 128 ? 7 : 6;
+    static_assert(TOKW == 1 << SHIFT, "query tiles of 64, 128 or 256 rows");
+    const PackedTile pt = packed_tile(p, number, SHIFT, PACK ? n_rep : 1, lane);
+    if (pt.tile < 0) return;
+    b = pt.b; qt = pt.tile;
+    q_first = pt.q_first; seg = pt.seg; k_first = pt.k_first; seg_k = pt.seg_k;
+    pk_tq = pt.tq; pk_ctx = pt.ctx;
+    stream_kv = PACK && pt.tiles == 1;
   } else {
     const int per_group = PACK ? nqt : nqt * hpg;
     stream_kv = PACK && nqt == 1;
@@ -220,12 +317,12 @@ void prefill_async_kernel(PrefillParams p) {
     seg = p.T; q_first = 0; k_first = 0; seg_k = 0;
   }
   const int kv0 = PAIR ? max(min(2 * hk, p.Hkv - 2), 0) : hk;    // first kv head of the rows' 256 bytes (PAIR: Hkv >= 2, checked on the host, but for `solo`)
-  const int hq = PACK ? hk * n_rep : kv0 * n_rep + QH * (rr_ % hpg);     // PACK: first head of the group; PAIR: the first kv head's; QH 2: and hq + 1
+  const int hq = PACK ? hk * n_rep : kv0 * n_rep + QH * (PACKED ? rr_ : rr_ % hpg);     // PACK: first head of the group; PAIR: the first kv head's; QH 2: and hq + 1
   const int half_heads = solo ? QH * hpg : n_rep;      // PAIR: q heads between the two halves' waves
   // row r of the workgroup (0 .. BMW-1) -> query token and q head
   const int v0 = qt * TOKW;
-  auto row_token = [&](int r) __attribute__((always_inline)) { return PACK ? (v0 + r) / n_rep : v0 + (PAIR ? (r & (TOKW - 1)) : r); };
-  auto row_head = [&](int r) __attribute__((always_inline)) { return PACK ? hq + (v0 + r) % n_rep : hq + (PAIR && r >= TOKW ? half_heads : 0); };
+  auto row_token = [&](int r) __attribute__((always_inline)) { return PACK ? (PACKED ? p.by_rep.quot(v0 + r) : (v0 + r) / n_rep) : v0 + (PAIR ? (r & (TOKW - 1)) : r); };
+  auto row_head = [&](int r) __attribute__((always_inline)) { return PACK ? hq + (PACKED ? p.by_rep.rem(v0 + r) : (v0 + r) % n_rep) : hq + (PAIR && r >= TOKW ? half_heads : 0); };
   const int par = PAIR ? wave / (NW / 2) : 0;   // which 128 bytes of the rows this wave works on
   const bool lone = PAIR && !solo && 2 * hk + 1 >= p.Hkv;     // the unpaired last head of an odd Hkv
   const bool solo_odd = solo && rr_ + hpg >= units;           // ... or an odd number of q heads (pairs) of a single kv head
@@ -234,11 +331,10 @@ void prefill_async_kernel(PrefillParams p) {
   // row of a query token in q and out
   auto token_row = [&](int t) __attribute__((always_inline)) -> long { return PACKED ? (long)q_first + t : (long)b * p.T + t; };
 
-  int tq = p.query_lens ? p.query_lens[b] : seg;
-  int ctx = p.seq_lens ? p.seq_lens[b] : PACKED ? seg_k : p.S;
-  tq = min(max(tq, 0), seg);
+  int tq = PACKED ? pk_tq : p.query_lens ? p.query_lens[b] : p.T;
+  int ctx = PACKED ? pk_ctx : p.seq_lens ? p.seq_lens[b] : p.S;
+  if (!PACKED) tq = min(max(tq, 0), p.T);
   if (MODE == 1) ctx = min(ctx, p.max_blocks * p.block_size);
-  if (PACKED) ctx = min(ctx, seg_k);
   ctx = max(ctx, 0);
   // more query tokens than context: the first ctx of them count, without a prefix (as pa_verify); packed rows keep the
   // alignment of the last query with the last key, and the first tq - ctx of them see nothing
@@ -639,8 +735,24 @@ void prefill_async_kernel(PrefillParams p) {
   // (sacc: NS 32-key sub-tiles that start at key key0; j: which head of the wave)
   auto softmax = [&](auto& sacc, auto& pw, int key0, int j) __attribute__((always_inline)) {
     constexpr int NS = sizeof(sacc) / sizeof(sacc[0]);
+    if (EXACT_Q) {
+#pragma unroll
+      for (int tt = 0; tt < NS; ++tt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sacc[tt][i] = fmaf(sacc[tt][i], sc, -m_ref[j]);
+    }
     const bool need_mask = key0 + 32 * NS - 1 > prefix + wq_lo;    // reaches past the first row's diagonal
-    if (need_mask) {
+    if (EXACT_Q && need_mask) {
+      // (opaque: left to itself the compiler takes the compares and selects of both branches onto every tile, a fourth
+      // of a tile's vector instructions)
+      int lim = qlim - key0 - 4 * h;
+      asm volatile("" : "+v"(lim));
+#pragma unroll
+      for (int tt = 0; tt < NS; ++tt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sacc[tt][i] = 32 * tt + 8 * (i >> 2) + (i & 3) <= lim ? sacc[tt][i] : -INFINITY;
+    }
+    if (!EXACT_Q && need_mask) {
       int kb = key0;
       // sub-tile form: keeps the key arithmetic and the compares inside the branch (the compiler hoisted them onto
       // every tile); the whole-tile forms do not need it, and with it they run out of registers
@@ -653,7 +765,15 @@ void prefill_async_kernel(PrefillParams p) {
           sacc[tt][i] = key <= qlim ? sacc[tt][i] : -INFINITY;
         }
     }
-    if (win > 0 && key0 < prefix + wq_hi - win + 1) {         // tile starts below the last row's window
+    if (EXACT_Q && win > 0 && key0 < prefix + wq_hi - win + 1) {
+      int lim = qlim - win + 1 - key0 - 4 * h;
+      asm volatile("" : "+v"(lim));
+#pragma unroll
+      for (int tt = 0; tt < NS; ++tt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sacc[tt][i] = 32 * tt + 8 * (i >> 2) + (i & 3) >= lim ? sacc[tt][i] : -INFINITY;
+    }
+    if (!EXACT_Q && win > 0 && key0 < prefix + wq_hi - win + 1) {         // tile starts below the last row's window
       const int qlo = qlim - win + 1;
       int kb = key0;
       if constexpr (NS == 1) asm volatile("" : "+s"(kb));       // (as above)
@@ -715,9 +835,11 @@ void prefill_async_kernel(PrefillParams p) {
       for (int tt = 0; tt < NS; ++tt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sacc[tt][i] -= shift;
-      const float neg_ref = -m_ref[j];
+      if (!EXACT_Q) {
+        const float neg_ref = -m_ref[j];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) asm volatile("v_mov_b32 %0, %1" : "+v"(cinit[j][i]) : "v"(neg_ref));
+        for (int i = 0; i < 16; ++i) asm volatile("v_mov_b32 %0, %1" : "+v"(cinit[j][i]) : "v"(neg_ref));
+      }
     }
     float psum = 0.f;
 #pragma unroll
@@ -776,7 +898,7 @@ void prefill_async_kernel(PrefillParams p) {
       uint32_t r[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        r[j] = pack_bf16x2(bf16_bits_to_float(w[j] & 0xffffu) * sc, bf16_bits_to_float(w[j] >> 16) * sc);
+        r[j] = EXACT_Q ? w[j] : pack_bf16x2(bf16_bits_to_float(w[j] & 0xffffu) * sc, bf16_bits_to_float(w[j] >> 16) * sc);
       qf[j][s] = make_frag(r[0], r[1], r[2], r[3]);
     }
     // the Q loads must be complete (and known to the compiler to be) before the loop, or the
@@ -886,6 +1008,12 @@ void prefill_async_kernel(PrefillParams p) {
           // registers hold besides the accumulators
 #pragma unroll
           for (int tt = 0; tt < TT; ++tt) {
+            // packed form: a sub-tile that no row of the wave sees -- past its last row's position, or under a sliding
+            // window in front of its first row's -- is passed over (window 128, 64 rows per workgroup: 5 to 6 of 8 are left)
+            if (PACKED && (w_c.kt * BN + 32 * tt > prefix + wq_hi || (win > 0 && w_c.kt * BN + 32 * tt + 31 < prefix + wq_lo - win + 1))) {
+              if (tt == 0) prefetch_next();
+              continue;
+            }
             bf16x8_t kf[KS];
             load_k(kf, stage_c, tt);
             f32x16_t sacc[QH][1];
@@ -1070,9 +1198,8 @@ hipError_t launch_typed(const PrefillParams& p, hipStream_t s) {
   const long groups = (long)p.B * (DH == 64 ? (p.Hkv + 1) / 2 : p.Hkv);
   long total = 8 * ((groups + 7) / 8) * per_group * (SPLIT ? p.splits : 1);
   if (MODE == 2) {       // the kernel's own numbering of (kv head, query tile, q head)
-    const int kvg = DH == 64 ? (p.Hkv + 1) / 2 : p.Hkv, units = n_rep / QH;
-    const long per_head = (long)p.slots * (PACK ? 1 : DH == 64 && p.Hkv == 1 ? (units + 1) / 2 : units);
-    const long items = kvg % 8 == 0 ? kvg / 8 * per_head : 8 % kvg == 0 ? (per_head * kvg + 7) / 8 : (per_head * kvg + 7) / 8;
+    const long per_head = (long)p.slots * p.hpg;
+    const long items = p.deal == 0 ? p.kvg / 8 * per_head : (per_head * p.kvg + 7) / 8;
     total = 8 * items * (SPLIT ? p.splits : 1);
   }
   if (total > 0x7fffffffL) return hipErrorInvalidValue;
@@ -1224,40 +1351,74 @@ hipError_t launch_prefill_async(const PrefillParams& p, int waves, hipStream_t s
 }
 
 // ---- packed form ---------------------------------------------------------------------------------------------
-// 128 packed rows of a kv group (its q heads ride along as rows of one tile), or 256 tokens of one q head
+// Workgroup shapes.  Head dim 64: 4 waves, 64 tokens of two kv heads (against 8 waves and 128 tokens, us: 16 windowed
+// prompts of 100-2 000 tokens 134 / 171, 32 prompts of 17-256 37 / 46, 2 of 4 097-8 192 891 / 965).  Head dim 128: 4 waves
+// with 128 rows of a kv group (its q heads' rows share the tile), two workgroups per CU, or 8 waves with 256 tokens of
+// one q head, one per CU: half the copies per product, for long prompts that fill the device twice over.  us, 4 / 8 waves,
+// 32 / 8 heads: 32 x 17-256 tokens 29.7 / 42, 8 x 500-1 024 56 / 66, 1 x 1 024 28.5 / 33, 8 x 2 048 319 / 321, 2 x 2 048
+// 85 / 78, 4 x 4 096 570 / 550, 1 x 8 192 538 / 512; 16 / 16 heads (nothing to share): 32 x 17-256 24 / 28, 4 x 500-2 000
+// 59.5 / 57.5, 4 x 4 096 293 / 281; a window of 1 024, 8 x 500-4 000: 310 / 331.
 static bool packed_takes_groups(const PrefillParams& p) {
-  return p.D == HD && p.impl != 8 && (p.impl == 5 || true);
+  if (p.D != HD || p.impl == 8) return false;
+  const long tokens = p.Hq == p.Hkv ? 1024 : 2048;      // on average per sequence
+  return p.impl == 5 || p.window > 0 || p.total_q < tokens * p.B || (long)p.total_q * p.Hq < 256L * 2 * p.num_cus;
 }
-static int packed_tile_shift(const PrefillParams& p) { return p.D == 64 || packed_takes_groups(p) ? 7 : 8; }
 static int packed_slots(const PrefillParams& p) {
-  const int mult = packed_takes_groups(p) ? p.Hq / p.Hkv : 1;
-  return (int)(((long)mult * p.total_q) >> packed_tile_shift(p)) + p.B;
+  const bool groups = packed_takes_groups(p);
+  const int mult = groups ? p.Hq / p.Hkv : 1;
+  const int shift = p.D == 64 ? 6 : groups ? 7 : 8;
+  return (int)(((long)mult * p.total_q) >> shift) + p.B;
+}
+static int packed_groups(const PrefillParams& p) { return p.D == 64 ? (p.Hkv + 1) / 2 : p.Hkv; }
+static int packed_heads_per_group(const PrefillParams& p) {      // workgroups per query tile and kv head (pair)
+  const int n_rep = p.Hq / p.Hkv, units = p.D == 64 ? n_rep / d64_heads_per_wave(p) : n_rep;
+  return packed_takes_groups(p) ? 1 : p.D == 64 && p.Hkv == 1 ? (units + 1) / 2 : units;
 }
 
 int prefill_packed_splits(const PrefillParams& p, int num_cus) {
-  (void)p; (void)num_cus;
-  return 1;
+  // few query tiles over many keys (a chunk behind a long prefix): the keys of a tile go to as many workgroups as fill
+  // the device, two per CU, at least eight key tiles each.  us, unsplit / the best number of shares, 32 / 8 heads of 128:
+  // 256 tokens behind 32 K 474 / 120 (8; with 4 137, with 16 133), 512 behind 4 K 74 / 47 (4; 2 54, 8 57), 64 behind 8 K 107 /
+  // 32 (16), 8 x 64 behind 8 K 161 / 79 (4); 64 / 8 heads of 64: 512 behind 4 K 106 / 53 (4), 256 behind 32 K 817 / 162 (8).
+  // A call that already has two workgroups for every three places is left alone (4 x 257-512 behind 4 K: 105 / 119 with two
+  // shares), and so are prompts with less than twice their length in front of them, which their own diagonal bounds
+  // (1 x 1 024: 28.5 / 35.5).
+  if (!packed_takes_groups(p) && p.D == HD) return 1;
+  const long bound = p.len_bound > 0 ? p.len_bound : p.total_k, mean = p.total_q / p.B;
+  if (bound < 3 * mean) return 1;
+  const int mult = p.D == HD ? p.Hq / p.Hkv : 1, shift = p.D == HD ? 7 : 6;
+  const long tiles = std::max(1L, (((long)mult * p.total_q) >> shift) + p.B / 2);      // about: the last tile of a sequence is half full
+  const long wgs = tiles * packed_groups(p) * packed_heads_per_group(p), places = 2L * num_cus;
+  const long s = std::min((2 * places + wgs) / (2 * wgs), bound / (8 * 64));
+  return s < 2 ? 1 : (int)std::min(s, 16L);
 }
 
 hipError_t launch_prefill_packed(const PrefillParams& p0, hipStream_t s) {
   PrefillParams p = p0;
   p.slots = packed_slots(p);
+  p.n_rep = p.Hq / p.Hkv;
+  p.kvg = packed_groups(p);
+  p.hpg = packed_heads_per_group(p);
+  p.deal = p.kvg % 8 == 0 ? 0 : 8 % p.kvg == 0 ? 8 / p.kvg : -1;
+  if ((long)p.slots * p.hpg > 0x7fffffffL) return hipErrorInvalidValue;
+  p.by_rep.set(p.n_rep); p.by_hpg.set(p.hpg); p.by_kvg.set(p.kvg); p.by_head.set(p.slots * p.hpg); p.by_splits.set(p.splits);
   const bool split = p.splits > 1;
   if (split && (!p.ws_o || !p.ws_ml)) return hipErrorInvalidValue;
   if (p.D == 64) {       // (window 0 included: see launch_prefill_async)
-    if (d64_heads_per_wave(p) == 2)
-      return split ? launch_typed<false, 2, 8, 2, true, false, true, false, 64, 2>(p, s)
-                   : launch_typed<false, 2, 8, 2, true, false, false, false, 64, 2>(p, s);
-    return split ? launch_typed<false, 2, 8, 2, true, false, true, false, 64>(p, s)
-                 : launch_typed<false, 2, 8, 2, true, false, false, false, 64>(p, s);
+    const bool two = d64_heads_per_wave(p) == 2;
+    if (two) return split ? launch_typed<false, 2, 4, 2, true, false, true, false, 64, 2>(p, s)
+                          : launch_typed<false, 2, 4, 2, true, false, false, false, 64, 2>(p, s);
+    return split ? launch_typed<false, 2, 4, 2, true, false, true, false, 64>(p, s)
+                 : launch_typed<false, 2, 4, 2, true, false, false, false, 64>(p, s);
   }
   if (p.D != HD) return hipErrorInvalidValue;
   if (packed_takes_groups(p)) {
     if (p.window > 0) return split ? launch_typed<false, 2, 4, 2, true, true, true>(p, s) : launch_typed<false, 2, 4, 2, true, true>(p, s);
     return split ? launch_typed<false, 2, 4, 2, false, true, true>(p, s) : launch_typed<false, 2, 4, 2, false, true>(p, s);
   }
-  if (p.window > 0) return split ? launch_typed<false, 2, 8, 2, true, false, true>(p, s) : launch_typed<false, 2, 8, 2, true>(p, s);
-  return split ? launch_typed<false, 2, 8, 2, false, false, true>(p, s) : launch_typed<false, 2, 8>(p, s);
+  // (the 8-wave form: dense long prompts that fill the device several times over; windows and splits are the other's)
+  if (p.window > 0 || split) return hipErrorInvalidValue;
+  return launch_typed<false, 2, 8>(p, s);
 }
 
 }  // namespace pa

@@ -85,8 +85,7 @@ def test_strided_rows(pa, rng, Hq, Hkv, D):
     _run(pa, rng, [100, 1, 200, 17], Hq, Hkv, D, strided=True)
 
 
-@pytest.mark.parametrize("impl", [0, 8])
-@pytest.mark.parametrize("split", [1, 0, 2, 5, 16])
+@pytest.mark.parametrize("impl,split", [(0, 1), (0, 0), (0, 2), (0, 5), (0, 16), (8, 0)])
 @pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (8, 2, 64), (3, 1, 64), (3, 3, 128)])
 def test_more_keys_than_queries_and_fewer(pa, rng, debug_switch, Hq, Hkv, D, split, impl):
     """Cached prefixes, sequences with fewer keys than queries (their first rows see nothing), and with none at all."""
