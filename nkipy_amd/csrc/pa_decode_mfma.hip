@@ -35,8 +35,9 @@
 // applied to the fp32 scores (K) and folded into P (V), so the dequantised
 // cache is never written anywhere.
 //
-// int8 KV: the same with a float32 scale per (token, kv head) and codes that a conversion to float32 and a
-// packing of high halves turn into bf16 (every code is a bf16 value).
+// int8 KV, with a float32 scale per (token, kv head): K's codes go into the integer matrix instruction as they lie, against
+// the query row as two 8-bit limbs (q_limbs); V's become bf16 by a conversion to float32 and a packing of high halves
+// (every code is a bf16 value), and the probabilities, times V's scale, go in as two bf16 terms.
 //
 // Math restated: attention.py:112-144 + softmax.py:4-6 in one pass; the merge
 // of partitions is  m = max m_i, l = sum l_i 2^(m_i-m), o = sum o_i l_i 2^(m_i-m)/l.
@@ -99,14 +100,14 @@ template <int D, int KV>
 struct KTile {
   static constexpr int KLD = KV != KV_BF16 ? D / 64 : D / 32;        // 16-byte K loads per 16-token sub-tile
   uint32_t k[2][KLD][4];
-  float ksc[KV == KV_I8 ? 8 : 2];      // fp8: scales of the two 16-token halves; int8: of the lane's eight tokens
+  float ksc[KV == KV_I8 ? 4 : 2];      // fp8: scales of the two 16-token halves; int8: see load_token_scales (K's and V's)
 };
 template <int D, int KV>
 struct VTile {
   static constexpr int VEC = D / 16;                                 // d's per lane for V
   static constexpr int VW = (VEC * (KV != KV_BF16 ? 1 : 2)) / 4;     // dwords per V load
   uint32_t v[8][VW];
-  float vsc[KV == KV_I8 ? 8 : 2];
+  float vsc[2];
 };
 
 // Per-wavefront streaming state: Q fragments, online-softmax state and output
@@ -171,6 +172,7 @@ struct DecodeWave {
   bf16x8_t qf[LEAN ? 1 : R][LEAN ? 1 : KSTEPS];
   uint4* qlds;               // LEAN: this wave's [R][KSTEPS][64] fragment store in LDS
   int qlane;                 // LEAN: lane index into it, re-made opaque per tile so the reads stay in the loop
+  float q_scale[I8 ? R : 1]; // int8: scale_log2e x the scale of this lane's query row (see q_limbs)
   bf16x8_t pf[R];            // P^T fragments of the current tile
   bf16x8_t pl[I8 ? R : 1];   // int8: what their rounding left over
   f32x4_t oacc[R][VEC];
@@ -364,6 +366,7 @@ struct DecodeWave {
           qraw[s].z = pack_bf16x2(x[s][4], x[s][5]); qraw[s].w = pack_bf16x2(x[s][6], x[s][7]);
         }
       }
+      if constexpr (I8) q_limbs(qraw, rg);
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
         if (LEAN) qlds[(rg * KSTEPS + s) * 64 + qlane] = qraw[s];
@@ -397,6 +400,59 @@ struct DecodeWave {
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) knew[s] = q.kraw[s];
     }
+  }
+
+  // int8: the row's values become 16-bit integers under a scale of their own, absmax / 32 512, in two limbs of 8 bits (256
+  // high + low, both signed): the score product is then the integer matrix instruction's on the codes as they lie in
+  // memory, exact, where a conversion to bf16 costs three vector instructions for two codes (64 / 8 heads of 128, 64
+  // sequences of 1 024-32 768 tokens: 203 -> 194 us, 6.0 TB/s; 64 / 8 heads of 64, 64 of 512-8 192: 80 -> 75.5).  An element is rounded at
+  // most half a step, 2^-16 of the row's largest; a bf16 value at least 2^-8 of the largest is not rounded at all.  Slot
+  // limb * KLD + s holds limb 0 (high) or 1 (low) of the 16 elements that lane (g, .) has of step s.  A row with an
+  // infinity or a NaN gets the scale NaN.
+  __device__ __forceinline__ void q_limbs(uint4 (&qraw)[KSTEPS], int rg) {
+    uint4 hq[KLD], lq[KLD];
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) {
+      const uint32_t w[4] = {qraw[s].x, qraw[s].y, qraw[s].z, qraw[s].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));      // (orders as the magnitudes do, a NaN above infinity)
+    }
+    top = over_g(top, [](uint32_t a, uint32_t b) __attribute__((always_inline)) { return max(a, b); });
+    // (reciprocals within an ulp do: absmax x inv rounds to 32 512 all the same, and the scale is inv's own)
+    const float inv = fminf(32512.f * __builtin_amdgcn_rcpf(__uint_as_float(top << 16)), 0x1p+120f);
+    q_scale[I8 ? rg : 0] = top >= 0x7f80u ? __uint_as_float(0x7fc00000u) : p.scale_log2e * __builtin_amdgcn_rcpf(inv);
+#pragma unroll
+    for (int s = 0; s < KLD; ++s) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        // x inv + 1.5 x 2^23: rounded to an integer, whose low 16 bits are the float's.  Its low byte is the low limb, the
+        // byte above it, after 128 is added, the high one.
+        const uint4& q4 = qraw[2 * s + (d >> 1)];
+        const uint32_t w0 = d & 1 ? q4.z : q4.x, w1 = d & 1 ? q4.w : q4.y;
+        const float x[4] = {__uint_as_float(w0 << 16), __uint_as_float(w0 & 0xffff0000u), __uint_as_float(w1 << 16), __uint_as_float(w1 & 0xffff0000u)};
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(fmaf(x[e], inv, 0x1.8p+23f));
+        lo[d] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], 0x0c0c0400u), __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u), 0x05040100u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += 128;
+        hi[d] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], 0x0c0c0501u), __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0501u), 0x05040100u);
+      }
+      hq[s] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      lq[s] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+#pragma unroll
+    for (int s = 0; s < KLD; ++s) { qraw[s] = hq[s]; qraw[KLD + s] = lq[s]; }
+  }
+  // f over the four lanes r, r + 16, r + 32, r + 48, in registers
+  template <class F>
+  static __device__ __forceinline__ uint32_t over_g(uint32_t v, F f) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t m = f(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    return f(b[0], b[1]);
   }
 
   // NEWROW: the raw K row -> knew, normed and rotated at position pos (the slow path of a token the call's length
@@ -443,17 +499,28 @@ struct DecodeWave {
   }
 
   // Token of the tile that slot j of this lane's eight score / probability / V-row slots stands for.  int8 pools keep
-  // the matrix instruction's own order, four consecutive tokens per lane and half, so that a lane's scales are two
-  // 16-byte loads (a scale per token, contiguous in the pool) instead of eight of 4 bytes.
+  // the matrix instruction's own order, four consecutive tokens per lane and half, so that a lane's scales are 16
+  // contiguous bytes per half.
   __device__ __forceinline__ int slot_token(int j) const { return I8 ? 16 * (j >> 2) + 4 * g + (j & 3) : 4 * j + g; }
-  // int8: scales [num_blocks, Hkv, block_size] of the lane's tokens of the tile at t0.  Those of tokens past the context
-  // are whatever the pool holds there; what they multiply is masked by selection.
-  __device__ __forceinline__ void load_token_scales(const float* tbl, float* sc, const TileRows& tr, int t0) const {
-    const int bmask = p.block_size - 1;
-    const float4 a = *(const float4*)(tbl + ((long)tr.blk0 * p.Hkv + hk) * p.block_size + (t0 & bmask) + 4 * g);
-    const float4 b = *(const float4*)(tbl + ((long)tr.blk1 * p.Hkv + hk) * p.block_size + ((t0 + 16) & bmask) + 4 * g);
+  // int8: the scales [num_blocks, Hkv, block_size] of the lane's tokens of the tile at t0, K's and V's, by one load
+  // instruction: the lanes r % 4 = 0, 1, 2, 3 fetch K's first and second half, V's first and second half, and the quad
+  // shares them (token_scale: a lane permutation that rides on the multiplication).  Four loads of every lane took 12
+  // registers more (some of which then spilled at head dim 128).  Scales of tokens past the context are whatever the pool holds there; what they multiply is masked by selection.
+  __device__ __forceinline__ void load_token_scales(float* sc, const TileRows& tr, int t0) const {
+    const bool second = r & 1;
+    const float* tbl = r & 2 ? p.v_scale : p.k_scale;
+    const int blk = second ? tr.blk1 : tr.blk0, at = (t0 + (second ? 16 : 0)) & (p.block_size - 1);
+    const float4 a = *(const float4*)(tbl + ((long)blk * p.Hkv + hk) * p.block_size + at + 4 * g);
     sc[0] = a.x; sc[1] = a.y; sc[2] = a.z; sc[3] = a.w;
-    sc[4] = b.x; sc[5] = b.y; sc[6] = b.z; sc[7] = b.w;
+  }
+  template <int FROM>        // the value of lane FROM of the quad
+  static __device__ __forceinline__ float of_quad(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), FROM * 0x55, 0xf, 0xf, true));
+  }
+  // K's (V false) or V's scale of slot j
+  template <bool V>
+  static __device__ __forceinline__ float token_scale(const float* sc, int j) {
+    return j < 4 ? of_quad<V ? 2 : 0>(sc[j & 3]) : of_quad<V ? 3 : 1>(sc[j & 3]);
   }
 
   // Loads of the tile starting at token t0.  Rows past the context are
@@ -465,7 +532,7 @@ struct DecodeWave {
       tl.ksc[0] = p.k_scale[(long)tr.blk0 * p.Hkv + hk];
       tl.ksc[1] = p.k_scale[(long)tr.blk1 * p.Hkv + hk];
     }
-    if (I8) load_token_scales(p.k_scale, tl.ksc, tr, t0);
+    if constexpr (I8) load_token_scales(tl.ksc, tr, t0);
     if (SK) {
       // One instruction = 8 rows x one whole 128-byte line (lane: row 8 hf + lane / 8 of the sub-tile in tile
       // order, 16-byte chunk lane % 8), so that a streamed line is used up by the instruction that fetches it; slot
@@ -521,7 +588,6 @@ struct DecodeWave {
       tl.vsc[0] = p.v_scale[(long)tr.blk0 * p.Hkv + hk];
       tl.vsc[1] = p.v_scale[(long)tr.blk1 * p.Hkv + hk];
     }
-    if (I8) load_token_scales(p.v_scale, tl.vsc, tr, t0);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int tl_ = min(slot_token(j), tr.lmax);
@@ -545,7 +611,28 @@ struct DecodeWave {
 #pragma unroll
     for (int rg = 0; rg < R; ++rg) sacc[rg][0] = sacc[rg][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     // each Q fragment is fetched once and used for both 16-token halves
-    if (!BYTES) {
+    if constexpr (I8) {
+      typedef int i32x4_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int rg = 0; rg < R; ++rg) {
+        i32x4_t hi[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, lo[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int s = 0; s < KLD; ++s) {
+          const i32x4_t qh = __builtin_bit_cast(i32x4_t, q_frag(rg, s)), ql = __builtin_bit_cast(i32x4_t, q_frag(rg, KLD + s));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const i32x4_t kc = {(int)tl.k[u][s][0], (int)tl.k[u][s][1], (int)tl.k[u][s][2], (int)tl.k[u][s][3]};
+            hi[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc, qh, hi[u], 0, 0, 0);
+            lo[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc, ql, lo[u], 0, 0, 0);
+          }
+        }
+        // (|256 high + low| <= 128 x 127 x 32 512 < 2^31)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sacc[rg][u][i] = (float)(256 * hi[u][i] + lo[u][i]);
+      }
+    } else if (!BYTES) {
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
 #pragma unroll
@@ -569,13 +656,8 @@ struct DecodeWave {
           k_chunk(tl, u, s, kc);
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
-            if (I8) {
-              w[u][2 * d] = pack_hi16(i8_to_float<0>(kc[d]), i8_to_float<1>(kc[d]));
-              w[u][2 * d + 1] = pack_hi16(i8_to_float<2>(kc[d]), i8_to_float<3>(kc[d]));
-            } else {
-              w[u][2 * d] = fp8x2_to_bf16x2<false>(kc[d]);
-              w[u][2 * d + 1] = fp8x2_to_bf16x2<true>(kc[d]);
-            }
+            w[u][2 * d] = fp8x2_to_bf16x2<false>(kc[d]);
+            w[u][2 * d + 1] = fp8x2_to_bf16x2<true>(kc[d]);
           }
         }
 #pragma unroll
@@ -594,14 +676,23 @@ struct DecodeWave {
       float sv[8];
       float tmax = -INFINITY;
       const int lim = MULTI ? min(t_end, row_end[rg]) : t_end;
+      if constexpr (I8) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float sc = FP8 ? p.scale_log2e * tl.ksc[u] : p.scale_log2e;
+        for (int i = 0; i < 8; ++i) sv[i] = sacc[rg][i >> 2][i & 3] * (q_scale[rg] * token_scale<false>(tl.ksc, i));
+        // (masks in a branch of their own, for the tiles that need them, measured slower: 64 / 8 heads of 128, 64
+        // sequences of 1 024-32 768 tokens 197 -> 227 us)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = t0 + slot_token(4 * u + i);
-          const float x = sacc[rg][u][i] * (I8 ? p.scale_log2e * tl.ksc[(4 * u + i) % (I8 ? 8 : 2)] : sc);
-          sv[4 * u + i] = tok < lim ? x : -INFINITY;
+        for (int i = 0; i < 8; ++i) sv[i] = t0 + slot_token(i) < lim ? sv[i] : -INFINITY;
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float sc = FP8 ? p.scale_log2e * tl.ksc[u] : p.scale_log2e;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tok = t0 + slot_token(4 * u + i);
+            const float x = sacc[rg][u][i] * sc;
+            sv[4 * u + i] = tok < lim ? x : -INFINITY;
+          }
         }
       }
       // sliding window: keys more than window - 1 tokens behind the row's own position are
@@ -614,8 +705,14 @@ struct DecodeWave {
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) tmax = fmaxf(tmax, sv[i]);
-      tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
-      tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+      if constexpr (I8) {
+        tmax = __uint_as_float(over_g(__float_as_uint(tmax), [](uint32_t a, uint32_t b) __attribute__((always_inline)) {
+          return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+        }));
+      } else {
+        tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
+        tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+      }
       const float m_new = fmaxf(m_run[rg], tmax);
       // MULTI: a row that has seen no key yet keeps m = -inf; exponents are then taken against 0
       const float m_ref = (MULTI && m_new == -INFINITY) ? 0.f : m_new;
@@ -634,9 +731,11 @@ struct DecodeWave {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { pr[i] *= vt.vsc[0]; pr[4 + i] *= vt.vsc[1]; }
       }
-      if (I8) {      // (a masked slot's scale may be anything, not a number included)
+      if constexpr (I8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pr[i] = sv[i] == -INFINITY ? 0.f : pr[i] * vt.vsc[i % (I8 ? 8 : 2)];
+        for (int i = 0; i < 8; ++i) pr[i] *= token_scale<true>(tl.ksc, i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pr[i] = sv[i] == -INFINITY ? 0.f : pr[i];      // a masked slot's scale may be anything, not a number included
       }
       const uint32_t pw[4] = {pack_bf16x2(pr[0], pr[1]), pack_bf16x2(pr[2], pr[3]), pack_bf16x2(pr[4], pr[5]), pack_bf16x2(pr[6], pr[7])};
       pf[rg] = as_bf16x8(pw[0], pw[1], pw[2], pw[3]);
