@@ -399,7 +399,8 @@ int pa_kv_write(const void* k_new, const void* v_new, void* k_cache, void* v_cac
 
 /* The same for packed rows: token t < query_lens[b] of sequence b is row cu_seqlens[b] + t of k_new / v_new
  * [total_tokens, Hkv, D] bf16, whose tokens lie k_stride / v_stride elements apart (multiples of 8, at least Hkv * D:
- * slices of a wider tensor).  At most cu_seqlens[b + 1] - cu_seqlens[b] rows of a sequence count; boundaries outside
+ * slices of a wider tensor).  A query length beyond the cu_seqlens[b + 1] - cu_seqlens[b] rows of a sequence counts as
+ * their number (as one beyond T does for pa_kv_write); boundaries outside
  * [0, total_tokens] count as its ends.  kv_dtype PA_BF16 or PA_INT8; D in {32, 64, 128, 256}. */
 int pa_kv_write_packed(const void* k_new, const void* v_new, long k_stride, long v_stride, const int32_t* cu_seqlens,
                        int total_tokens, void* k_cache, void* v_cache, float* k_scale, float* v_scale,

@@ -137,7 +137,7 @@ using namespace pa;
 
 extern "C" {
 
-int pa_version(void) { return 300; }   // 0.3.0: pa_prefill takes max_seq_len; the one-call steps; sinks and windows on small calls
+int pa_version(void) { return 400; }   // 0.4.0: int8 pools, pa_kv_write_packed, pa_read_kv, pa_packed_prefill
 
 const char* pa_last_error(void) { return tl_error; }
 

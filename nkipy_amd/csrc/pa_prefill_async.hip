@@ -1185,12 +1185,15 @@ template <bool SPARSE, int MODE, int NW, int TT = 2, bool WIN = false, bool PACK
 hipError_t launch_typed(const PrefillParams& p, hipStream_t s) {
   constexpr int lds = (SPARSE && NW == 8 ? 5 : NW == 8 ? 4 : 2) * 2 * 32 * TT * ROW_B;
   constexpr int TOKW = DH == 64 ? 16 * NW : 32 * NW;      // query tokens per workgroup (plain form)
-  static std::atomic<int> configured{0};
-  if (!configured.load(std::memory_order_acquire)) {
+  static std::atomic<unsigned long long> configured{0};       // a bit per device: the attribute belongs to the device's own copy of the kernel
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) { (void)hipGetLastError(); dev = 0; }
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load(std::memory_order_acquire) & bit)) {
     hipError_t e = hipFuncSetAttribute((const void*)prefill_async_kernel<SPARSE, MODE, NW, TT, WIN, PACK, SPLIT, FP8, DH, QH>,
                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
-    configured.store(1, std::memory_order_release);
+    configured.fetch_or(bit, std::memory_order_release);
   }
   const int n_rep = p.Hq / p.Hkv;
   const long per_group = PACK ? ((long)p.T * n_rep + 32 * NW - 1) / (32 * NW)

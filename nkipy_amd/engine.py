@@ -7,8 +7,8 @@ role needs three small pieces:
 
 * `BlockAllocator`  -- free list with reference counts (a block shared by a forked prefix
                        is freed when its last user goes);
-* `PagedKVCache`    -- the K/V pools of the model's layers (bf16, or fp8-e4m3 with
-                       per-(block, kv head) scales), the per-slot block lists and the
+* `PagedKVCache`    -- the K/V pools of the model's layers (bf16, fp8-e4m3 with
+                       per-(block, kv head) scales, or int8 with per-(token, kv head) ones), the per-slot block lists and the
                        device-resident `block_tables` / `seq_lens` the kernels read; the
                        layers share the tables, as the reference's layers share start_pos
                        (examples/models/qwen3/qwen3.py:310-336), so a step reserves blocks
@@ -88,14 +88,17 @@ class PagedKVCache:
     seq_len 0 is idle.  Every layer has its own pool `k_caches[l]` / `v_caches[l]`; block ids, tables
     and lengths are common to all layers.  `dtype` torch.bfloat16, or torch.float8_e4m3fn (then
     `k_scales[l]` / `v_scales[l]` [num_blocks, Hkv] float32 exist and are maintained by the write
-    kernel).  `k_cache`, `v_cache`, `k_scale`, `v_scale` name layer 0.
+    kernel), or torch.int8 (scales [num_blocks, Hkv, block_size] float32, one per token and kv head; head_dim 64 or
+    128, a power-of-two block size >= 16).  `k_cache`, `v_cache`, `k_scale`, `v_scale` name layer 0.
     """
 
     def __init__(self, num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int, *, max_seqs: int,
                  max_blocks_per_seq: int, dtype=torch.bfloat16, device="cuda", num_layers: int = 1,
                  max_model_len: Optional[int] = None):
-        if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+        if dtype not in (torch.bfloat16, torch.float8_e4m3fn, torch.int8):
             raise ValueError(f"unsupported pool dtype {dtype}")
+        if dtype == torch.int8 and not paged_attn.verify_supported(1, head_dim, block_size):
+            raise ValueError(f"an int8 cache needs head_dim 64 or 128 and a power-of-two block size >= 16, got {head_dim} and {block_size}")
         if num_layers < 1:
             raise ValueError("num_layers must be at least 1")
         # the longest sequence a slot may grow to: the table capacity (whole blocks) unless the model's own limit is
@@ -108,7 +111,7 @@ class PagedKVCache:
         self.max_seqs, self.max_blocks_per_seq, self.num_layers = max_seqs, max_blocks_per_seq, num_layers
         self.device = torch.device(device)
         shape = (num_blocks, block_size, n_kv_heads, head_dim)
-        fp8 = dtype == torch.float8_e4m3fn
+        fp8, self.int8 = dtype == torch.float8_e4m3fn, dtype == torch.int8
 
         def pool():
             if fp8:
@@ -116,6 +119,8 @@ class PagedKVCache:
             return torch.zeros(shape, dtype=dtype, device=device)
 
         def scales():
+            if self.int8:
+                return torch.zeros((num_blocks, n_kv_heads, block_size), dtype=torch.float32, device=device)
             return torch.zeros((num_blocks, n_kv_heads), dtype=torch.float32, device=device) if fp8 else None
 
         self.k_caches = [pool() for _ in range(num_layers)]
@@ -136,15 +141,20 @@ class PagedKVCache:
         n_tab = max_seqs * max_blocks_per_seq
         self._off_lens = (n_tab + 63) // 64 * 64
         self._off_qlens = self._off_lens + (max_seqs + 63) // 64 * 64
-        self._host_meta = np.zeros(self._off_qlens + max_seqs, dtype=np.int32)
+        # int8 caches: where each slot's context begins among the rows of all slots that take part in the step, for the
+        # chunks that read the cache back (PagedAttention.attend)
+        self._off_starts = self._off_qlens + ((max_seqs + 63) // 64 * 64 if self.int8 else max_seqs)
+        self._host_meta = np.zeros(self._off_starts + (max_seqs + 1 if self.int8 else 0), dtype=np.int32)
         self._host_tables = self._host_meta[:n_tab].reshape(max_seqs, max_blocks_per_seq)
         self._host_tables[:] = -1
         self._host_lens = self._host_meta[self._off_lens:self._off_lens + max_seqs]
-        self._host_qlens = self._host_meta[self._off_qlens:]
+        self._host_qlens = self._host_meta[self._off_qlens:self._off_qlens + max_seqs]
+        self._host_starts = self._host_meta[self._off_starts:]
         self._meta = torch.from_numpy(self._host_meta).to(self.device)
         self.block_tables = self._meta[:n_tab].view(max_seqs, max_blocks_per_seq)
         self.seq_lens = self._meta[self._off_lens:self._off_lens + max_seqs]
-        self.query_lens = self._meta[self._off_qlens:]
+        self.query_lens = self._meta[self._off_qlens:self._off_qlens + max_seqs]
+        self.row_starts = self._meta[self._off_starts:] if self.int8 else None
         self._stage = self._stage_done = None
         self._stage_at = 0
         if self.device.type == "cuda":
@@ -231,6 +241,8 @@ class PagedKVCache:
         """Host mirror -> device (tables, lengths, query lengths: one copy, queued on the current stream)."""
         for s in slots:
             self._host_lens[s] = self.lens[s]
+        if self.int8:
+            np.cumsum(np.where(self._host_qlens > 0, self._host_lens, 0), out=self._host_starts[1:])
         if self._stage is None:
             self._meta.copy_(torch.from_numpy(self._host_meta))
             return
@@ -257,7 +269,8 @@ class PagedAttention:
     projected q/k/v of every slot, [max_seqs, T, H, D] bfloat16 (slot b contributes its first
     query_lens[b] rows; idle slots 0).  `attend` applies the optional QK RMSNorm + RoPE, writes K/V
     into the layer's pool and runs the prefill / verify kernel (T > 1) or the decode kernel
-    (T == 1).  Returns [max_seqs, T, Hq, D] (a preallocated buffer, overwritten by the next step of
+    (T == 1); over an int8 cache a long chunk reads the contexts back as bfloat16 rows (`read_kv`) and attends to those
+    (`packed_prefill`).  Returns [max_seqs, T, Hq, D] (a preallocated buffer, overwritten by the next step of
     the same T), or, when the layer was given `o_weight`, the output projection of it, [max_seqs, T, hidden].
 
     `attend` makes no host synchronisation and, after the first call of a given T, no allocation, so the
@@ -311,6 +324,8 @@ class PagedAttention:
             raise ValueError(f"o_weight must be [{n_heads * cache.head_dim}, hidden], got {tuple(o_weight.shape)}")
         self._out: Dict[int, torch.Tensor] = {}
         self._proj: Dict[int, torch.Tensor] = {}
+        self._q: Dict[int, torch.Tensor] = {}            # chunks over an int8 cache: transformed queries, first rows
+        self._starts: Dict[int, torch.Tensor] = {}
         # decode / verify steps prepared once per (T, length bound, storage of xq / xk / xv): a loop that feeds the
         # layer from the same buffers every step pays the argument checks once (see paged_attn.PreparedStep)
         self._steps: Dict[tuple, tuple] = {}
@@ -414,6 +429,8 @@ class PagedAttention:
 
             self._prepared(T, bound, xq, xk, xv, make).launch()
             return res
+        if c.int8:
+            return self._attend_read_back(xq, xk, xv, out, bound, capturing)
         qt = None
         if self.rope is not None:
             # the Q half of the norm and rotation rides on the attention kernel's Q load where that
@@ -443,6 +460,39 @@ class PagedAttention:
             paged_attn.prefill(q, kc, vc, c.block_tables, c.seq_lens, c.query_lens, self.scale,
                                k_scale=ks, v_scale=vs, out=out, max_seq_len=bound,
                                sinks=self.sinks, sliding_window=self.sliding_window, q_transform=qt)
+        if self.o_weight is None:
+            return out
+        proj = self._proj.get(T)
+        if proj is None:
+            proj = self._proj[T] = torch.empty((B, T, self.o_weight.shape[1]), dtype=torch.bfloat16, device=c.device)
+        return paged_attn.o_proj(out, self.o_weight, self.o_bias, out=proj)
+
+    def _attend_read_back(self, xq, xk, xv, out, bound, capturing):
+        """A chunk too long for the verify kernel over an int8 cache: write, read the contexts of the slots that take part
+        back as bfloat16 rows, attend to them.  A prompt in chunks and in one piece sees the same, quantised, keys."""
+        c, l = self.cache, self.layer
+        B, T = xq.shape[:2]
+        kc, vc, ks, vs = c.k_caches[l], c.v_caches[l], c.k_scales[l], c.v_scales[l]
+        if self.rope is not None:
+            q = self._q.get(T)
+            if q is None:
+                q = self._q[T] = torch.empty_like(xq)
+            q = paged_attn.qk_norm_rope_kv_write(xq, xk, xv, kc, vc, c.block_tables, c.seq_lens, c.query_lens, self.rope[0], self.rope[1],
+                                                 q_norm_weight=self.q_norm_weight, k_norm_weight=self.k_norm_weight,
+                                                 eps=self.norm_eps, k_scale=ks, v_scale=vs, out=q)
+        else:
+            paged_attn.kv_write(xk, xv, kc, vc, c.block_tables, c.seq_lens, c.query_lens, k_scale=ks, v_scale=vs)
+            q = xq
+        starts = self._starts.get(T)
+        if starts is None:
+            starts = self._starts[T] = torch.arange(0, (B + 1) * T, T, dtype=torch.int32, device=c.device)
+        # rows for the contexts: what the host knows of this step, or, captured into a graph that will be replayed on
+        # other lengths, what the bound admits
+        rows = B * bound if capturing else int(c._host_starts[-1])
+        k, v = paged_attn.read_kv(kc, vc, c.block_tables, c.seq_lens, c.row_starts, rows, k_scale=ks, v_scale=vs)
+        paged_attn.packed_prefill(q.reshape(B * T, self.n_heads, c.head_dim), k, v, starts, self.scale, cu_seqlens_k=c.row_starts,
+                                  query_lens=c.query_lens, seq_lens=c.seq_lens, max_seq_len=bound, sinks=self.sinks,
+                                  sliding_window=self.sliding_window, out=out.view(B * T, self.n_heads, c.head_dim))
         if self.o_weight is None:
             return out
         proj = self._proj.get(T)

@@ -47,6 +47,8 @@ def _need_device(name, t):
 
 
 def _check(cond, msg):
+    # (the calls a decode loop issues by the thousand spell the raise out where the text is formatted: an argument is
+    # formatted whether it is needed or not, and a dozen of them were a quarter of a small call's host time)
     if not cond:
         raise ValueError(msg)
 
@@ -88,7 +90,8 @@ def _on(device):
 
 
 def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+    """A tensor's address as the C signatures take it (a plain int: wrapping it costs as much again)."""
+    return t.data_ptr() if t is not None else None
 
 
 def _raise_on(rc, what):
@@ -100,7 +103,8 @@ def _kv_code(cache, scale_given):
     if cache.dtype == torch.uint8:
         _check(scale_given, "uint8 KV caches are fp8-e4m3fn codes and need k_scale/v_scale")
         return FP8
-    _check(cache.dtype in _DTYPE_CODE, f"unsupported KV cache dtype {cache.dtype}")
+    if cache.dtype not in _DTYPE_CODE:
+        raise ValueError(f"unsupported KV cache dtype {cache.dtype}")
     return _DTYPE_CODE[cache.dtype]
 
 
@@ -108,11 +112,12 @@ def _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, what="
     """The scale tables of a pool of codes: one float per (block, kv head) for fp8, per (token, kv head) for int8."""
     shape, text = ((num_blocks, Hkv), "[num_blocks, Hkv]") if kv_code == FP8 else \
                   ((num_blocks, Hkv, block_size), "[num_blocks, Hkv, block_size]")
-    _check(k_scale is not None and v_scale is not None,
-           f"{'fp8' if kv_code == FP8 else 'int8'} {what} needs both k_scale and v_scale")
+    if not (k_scale is not None and v_scale is not None):
+        raise ValueError(f"{'fp8' if kv_code == FP8 else 'int8'} {what} needs both k_scale and v_scale")
     for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
         _need_device(n, t)
-        _check(t.dtype == torch.float32 and t.shape == shape, f"{n} must be float32 {text}")
+        if not (t.dtype == torch.float32 and t.shape == shape):
+            raise ValueError(f"{n} must be float32 {text}")
 
 
 def _check_paging(k_cache, v_cache, block_tables, seq_lens, B):
@@ -269,28 +274,35 @@ def decode(q, k_cache, v_cache, block_tables, seq_lens, scale, *, k_scale=None, 
         _need_device(n, t)
     _check(q.dim() == 3, "q must be [B, Hq, D]")
     B, Hq, D = q.shape
-    _check(q.dtype in (torch.float32, torch.bfloat16), f"unsupported q dtype {q.dtype}")
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"unsupported q dtype {q.dtype}")
     _check_paging(k_cache, v_cache, block_tables, seq_lens, B)
     num_blocks, block_size, Hkv, Dk = k_cache.shape
-    _check(Dk == D, f"head_dim mismatch: q has {D}, cache has {Dk}")
-    _check(Hq % Hkv == 0, f"Hq={Hq} is not a multiple of Hkv={Hkv}")
-    _check(D in (32, 64, 128, 256), f"head_dim {D} not in (32, 64, 128, 256)")
+    if Dk != D:
+        raise ValueError(f"head_dim mismatch: q has {D}, cache has {Dk}")
+    if Hq % Hkv != 0:
+        raise ValueError(f"Hq={Hq} is not a multiple of Hkv={Hkv}")
+    if D not in (32, 64, 128, 256):
+        raise ValueError(f"head_dim {D} not in (32, 64, 128, 256)")
     scaled = k_scale is not None or v_scale is not None
     kv_code = _kv_code(k_cache, scaled)
     q_code = _DTYPE_CODE[q.dtype]
     if kv_code in (FP8, I8):
-        _check(q_code == BF16, f"{'fp8' if kv_code == FP8 else 'int8'} KV needs bfloat16 q")
+        if q_code != BF16:
+            raise ValueError(f"{'fp8' if kv_code == FP8 else 'int8'} KV needs bfloat16 q")
         _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv)
-        _check(kv_code == FP8 or verify_supported(1, D, block_size),
-               f"int8 KV needs head_dim 64 or 128 and a power-of-two block size >= 16 (D={D}, block_size={block_size})")
+        if not (kv_code == FP8 or verify_supported(1, D, block_size)):
+            raise ValueError(f"int8 KV needs head_dim 64 or 128 and a power-of-two block size >= 16 (D={D}, block_size={block_size})")
     else:
-        _check(kv_code == q_code, f"KV dtype {k_cache.dtype} does not match q dtype {q.dtype}")
+        if kv_code != q_code:
+            raise ValueError(f"KV dtype {k_cache.dtype} does not match q dtype {q.dtype}")
         _check(not scaled, "k_scale/v_scale are only valid with an fp8 or int8 KV cache")
     sinks, win = _check_variant(sinks, sliding_window, Hq, q)
     _check(isinstance(partition_size, int) and partition_size > 0, "partition_size must be a positive int")
     cap = block_tables.shape[1] * block_size
     msl = cap if max_seq_len is None else int(max_seq_len)
-    _check(0 < msl <= cap, f"max_seq_len {msl} outside (0, {cap}]")
+    if not (0 < msl <= cap):
+        raise ValueError(f"max_seq_len {msl} outside (0, {cap}]")
     _same_device(q, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables, seq_lens=seq_lens,
                  k_scale=k_scale, v_scale=v_scale, out=out)
     if validate_tables:
@@ -300,17 +312,17 @@ def decode(q, k_cache, v_cache, block_tables, seq_lens, scale, *, k_scale=None, 
     else:
         _need_device("out", out)
         _check(out.shape == q.shape and out.dtype == q.dtype, "out must match q in shape and dtype")
-    with _on(q.device):
-        need = int(lib.pa_decode_workspace_bytes_for(B, Hq, Hkv, D, block_size, msl, partition_size, q_code, kv_code))
-    stream = _stream_ptr(q.device)
-    if workspace is None:
-        workspace = _workspace(q.device, need, stream) if need else None
-    else:
-        _need_device("workspace", workspace)
-        _check(workspace.numel() * workspace.element_size() >= need, f"workspace needs {need} bytes")
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     qt_keep, qt_ptr = _qt_arg(q_transform, D, q)
     with _on(q.device):
+        need = int(lib.pa_decode_workspace_bytes_for(B, Hq, Hkv, D, block_size, msl, partition_size, q_code, kv_code))
+        stream = _stream_ptr(q.device)
+        if workspace is None:
+            workspace = _workspace(q.device, need, stream) if need else None
+        else:
+            _need_device("workspace", workspace)
+            if workspace.numel() * workspace.element_size() < need:
+                raise ValueError(f"workspace needs {need} bytes")
+        ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
         rc = lib.pa_decode(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
                            _ptr(block_tables), _ptr(seq_lens), _ptr(out), _ptr(workspace), ws_bytes,
                            B, Hq, Hkv, D, block_size, block_tables.shape[1], num_blocks, msl,
@@ -407,8 +419,10 @@ def prefill(q, k_cache, v_cache, block_tables, seq_lens, query_lens, scale, *, k
     _check(kv_code in (BF16, FP8, I8), "prefill needs a bfloat16, fp8 or int8 KV cache")
     _check(query_lens.shape == (B,) and query_lens.dtype == torch.int32, "query_lens must be int32 [B]")
     num_blocks, block_size, Hkv, Dk = k_cache.shape
-    _check(Dk == D, f"head_dim mismatch: q has {D}, cache has {Dk}")
-    _check(Hq % Hkv == 0, f"Hq={Hq} is not a multiple of Hkv={Hkv}")
+    if Dk != D:
+        raise ValueError(f"head_dim mismatch: q has {D}, cache has {Dk}")
+    if Hq % Hkv != 0:
+        raise ValueError(f"Hq={Hq} is not a multiple of Hkv={Hkv}")
     if kv_code in (FP8, I8):
         _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv)
     else:
@@ -418,16 +432,17 @@ def prefill(q, k_cache, v_cache, block_tables, seq_lens, query_lens, scale, *, k
     can_verify = verify_supported(T, D, block_size)
     if kv_code == I8:
         # only the decode-shaped kernel reads int8 pools: long query runs read the pool back (read_kv) for packed_prefill
-        _check(route != "tiled" and can_verify,
-               f"prefill over an int8 pool takes runs of up to 64 tokens (the verify kernel: head_dim 64 or 128, a power-of-two "
-               f"block size >= 16; T={T}, D={D}, block_size={block_size}); longer ones go through read_kv and packed_prefill")
+        if not (route != "tiled" and can_verify):
+            raise ValueError(f"prefill over an int8 pool takes runs of up to 64 tokens (the verify kernel: head_dim 64 or 128, a power-of-two "
+                             f"block size >= 16; T={T}, D={D}, block_size={block_size}); longer ones go through read_kv and packed_prefill")
         route = "verify"
     if route is None:
         route = prefill_route(B, T, Hq, Hkv, D, block_size, kv_code == FP8, win,
                               None if max_seq_len is None else int(max_seq_len))
     if route == "verify":
-        _check(can_verify, f"the verify kernel needs T <= 64, head_dim 64 or 128 and a power-of-two block size >= 16 "
-                           f"(T={T}, D={D}, block_size={block_size})")
+        if not (can_verify):
+            raise ValueError(f"the verify kernel needs T <= 64, head_dim 64 or 128 and a power-of-two block size >= 16 "
+                             f"(T={T}, D={D}, block_size={block_size})")
     _same_device(q, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables, seq_lens=seq_lens,
                  query_lens=query_lens, k_scale=k_scale, v_scale=v_scale, out=out)
     if validate_tables:
@@ -441,14 +456,16 @@ def prefill(q, k_cache, v_cache, block_tables, seq_lens, query_lens, scale, *, k
     stream = _stream_ptr(q.device)
     cap = block_tables.shape[1] * block_size
     msl = 0 if max_seq_len is None else int(max_seq_len)
-    _check(max_seq_len is None or 0 < msl <= cap, f"max_seq_len {msl} outside (0, {cap}]")
+    if not (max_seq_len is None or 0 < msl <= cap):
+        raise ValueError(f"max_seq_len {msl} outside (0, {cap}]")
     if route == "verify":
         need = int(lib.pa_verify_workspace_bytes(B, T, Hq, D))
         if workspace is None:
             workspace = _workspace(q.device, need, stream)
         else:
             _need_device("workspace", workspace)
-            _check(workspace.numel() * workspace.element_size() >= need, f"workspace needs {need} bytes")
+            if workspace.numel() * workspace.element_size() < need:
+                raise ValueError(f"workspace needs {need} bytes")
         ws_bytes = workspace.numel() * workspace.element_size()
         with _on(q.device):
             rc = lib.pa_verify(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
@@ -464,7 +481,8 @@ def prefill(q, k_cache, v_cache, block_tables, seq_lens, query_lens, scale, *, k
             workspace = _workspace(q.device, need, stream) if need else None
         else:
             _need_device("workspace", workspace)
-            _check(workspace.numel() * workspace.element_size() >= need, f"workspace needs {need} bytes")
+            if workspace.numel() * workspace.element_size() < need:
+                raise ValueError(f"workspace needs {need} bytes")
         ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
         rc = lib.pa_prefill(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
                             _ptr(block_tables), _ptr(seq_lens),
@@ -534,8 +552,8 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
     seq_lens[i] keys (rows laid out with room to spare); the other query rows are padding, zero in the result, and the
     other keys are never read.  A query that sees no key gets zeros; rows that belong to no sequence are left as they
     are (whatever the memory held in a result allocated here).
-    K and V rows are expected to be finite: a V row with an infinity or a NaN reaches the rows of up to 255 queries
-    in front of it as well (their weight for it is 0, and 0 x inf is not).
+    K and V rows are expected to be finite: a V row with an infinity or a NaN can reach the rows of up to 95
+    queries in front of it as well (their weight for it is 0, and 0 x inf is not).
     max_seq_len: host-known upper bound of a sequence's keys; sizes the split of calls with few queries over many keys
     (default Nk).  sinks [Hq] / sliding_window as in `decode`, the window counted back from each query.
     """
@@ -544,29 +562,35 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
     Nq, Hq, D = q.shape
     Nk, Hkv = k.shape[:2]
     _check(k.shape[2] == D and v.shape == k.shape, "k and v must be [Nk, Hkv, D] with q's D")
-    _check(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"Hq={Hq} is not a multiple of Hkv={Hkv}")
-    _check(D in (64, 128), f"head_dim {D} must be 64 or 128")
+    if not (Hkv > 0 and Hq > 0 and Hq % Hkv == 0):
+        raise ValueError(f"Hq={Hq} is not a multiple of Hkv={Hkv}")
+    if D not in (64, 128):
+        raise ValueError(f"head_dim {D} must be 64 or 128")
     _need_device("cu_seqlens", cu_seqlens)
     _check(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "cu_seqlens must be int32 [num_seqs + 1]")
     S = cu_seqlens.shape[0] - 1
     _check_cu("cu_seqlens", cu_seqlens, S)
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens
-        _check(Nk == Nq, f"k has {Nk} rows, q {Nq}: give cu_seqlens_k")
+        if Nk != Nq:
+            raise ValueError(f"k has {Nk} rows, q {Nq}: give cu_seqlens_k")
     else:
         _check_cu("cu_seqlens_k", cu_seqlens_k, S)
     for n, t in (("query_lens", query_lens), ("seq_lens", seq_lens)):
         if t is not None:
             _need_device(n, t)
-            _check(t.shape == (S,) and t.dtype == torch.int32, f"{n} must be int32 [num_seqs]")
-    _check(max_seq_len is None or int(max_seq_len) > 0, f"max_seq_len {max_seq_len} must be positive")
+            if not (t.shape == (S,) and t.dtype == torch.int32):
+                raise ValueError(f"{n} must be int32 [num_seqs]")
+    if not (max_seq_len is None or int(max_seq_len) > 0):
+        raise ValueError(f"max_seq_len {max_seq_len} must be positive")
     bound = Nk if max_seq_len is None else min(int(max_seq_len), Nk)
     sinks, win = _check_variant(sinks, sliding_window, Hq, q)
     if out is None:
         out = torch.empty((Nq, Hq, D), dtype=torch.bfloat16, device=q.device)
     else:
         _need_device("out", out)
-        _check(tuple(out.shape) == (Nq, Hq, D) and out.dtype == torch.bfloat16, f"out must be bfloat16 {(Nq, Hq, D)}")
+        if not (tuple(out.shape) == (Nq, Hq, D) and out.dtype == torch.bfloat16):
+            raise ValueError(f"out must be bfloat16 {(Nq, Hq, D)}")
     _same_device(q, k=k, v=v, cu_seqlens=cu_seqlens, cu_seqlens_k=cu_seqlens_k, query_lens=query_lens, seq_lens=seq_lens, out=out)
     with _on(q.device):
         stream = _stream_ptr(q.device)
@@ -581,7 +605,8 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
         else:
             _need_device("workspace", workspace)
             _same_device(q, workspace=workspace)
-            _check(workspace.numel() * workspace.element_size() >= need, f"workspace needs {need} bytes")
+            if workspace.numel() * workspace.element_size() < need:
+                raise ValueError(f"workspace needs {need} bytes")
         ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
         rc = lib.pa_packed_prefill(_ptr(q), _ptr(k), _ptr(v), qs, ks, vs, _ptr(cu_seqlens), _ptr(cu_seqlens_k), _ptr(query_lens),
                                    _ptr(seq_lens), _ptr(out), _ptr(workspace), ws_bytes, S, Nq, Nk, Hq, Hkv, D, bound,
@@ -607,7 +632,8 @@ def gather_kv(cache, block_tables, seq_lens, max_seq_len=None):
     num_blocks, block_size, Hkv, D = cache.shape
     cap = block_tables.shape[1] * block_size
     msl = cap if max_seq_len is None else int(max_seq_len)
-    _check(0 <= msl <= cap, f"max_seq_len {msl} outside [0, {cap}]")
+    if not (0 <= msl <= cap):
+        raise ValueError(f"max_seq_len {msl} outside [0, {cap}]")
     out = torch.empty((B, msl, Hkv, D), dtype=cache.dtype, device=cache.device)
     with _on(cache.device):
         rc = lib.pa_gather_kv(_ptr(cache), _ptr(block_tables), _ptr(seq_lens), _ptr(out), B, Hkv, D,
@@ -621,22 +647,27 @@ def _token_rows(name, t, dtype=torch.bfloat16):
     """Packed rows [tokens, heads, D] on the device whose tokens may lie apart (a slice of a wider projection output): the
     heads and their elements are adjacent, and the token stride is a multiple of 8 elements.  Returns the token stride."""
     if isinstance(t, torch.Tensor) and t.is_cuda and not t.is_contiguous():
-        _check(t.dim() == 3, f"{name} must be [tokens, heads, D]")
-        _check((t.stride(2) == 1 or t.shape[2] == 1) and (t.stride(1) == t.shape[2] or t.shape[1] == 1),
-               f"{name}: the heads of a token must be adjacent rows of D elements (strides {t.stride()})")
-        _check(t.stride(0) % 8 == 0 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1] * t.shape[2]),
-               f"{name}: the token stride {t.stride(0)} must be a multiple of 8 elements and at least a token's row")
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [tokens, heads, D]")
+        if not ((t.stride(2) == 1 or t.shape[2] == 1) and (t.stride(1) == t.shape[2] or t.shape[1] == 1)):
+            raise ValueError(f"{name}: the heads of a token must be adjacent rows of D elements (strides {t.stride()})")
+        if not (t.stride(0) % 8 == 0 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1] * t.shape[2])):
+            raise ValueError(f"{name}: the token stride {t.stride(0)} must be a multiple of 8 elements and at least a token's row")
     else:
         _need_device(name, t)
-        _check(t.dim() == 3, f"{name} must be [tokens, heads, D]")
-    _check(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
-    _check(t.data_ptr() % 16 == 0, f"{name} must start on a 16-byte boundary")
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [tokens, heads, D]")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.data_ptr() % 16 != 0:
+        raise ValueError(f"{name} must start on a 16-byte boundary")
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
 def _check_cu(name, cu, n):
     _need_device(name, cu)
-    _check(cu.dim() == 1 and cu.dtype == torch.int32 and cu.shape[0] == n + 1, f"{name} must be int32 [{n + 1}]: where each sequence's rows begin")
+    if not (cu.dim() == 1 and cu.dtype == torch.int32 and cu.shape[0] == n + 1):
+        raise ValueError(f"{name} must be int32 [{n + 1}]: where each sequence's rows begin")
 
 
 def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens, *, k_scale=None, v_scale=None, cu_seqlens=None):
@@ -655,8 +686,8 @@ def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens,
     gets the scale NaN: it reads back as NaN.
 
     cu_seqlens int32 [B + 1]: the new rows come packed, k_new/v_new [tokens, Hkv, D] bfloat16 with token t of
-    sequence b in row cu_seqlens[b] + t (bfloat16 and int8 pools); at most the cu_seqlens[b + 1] -
-    cu_seqlens[b] rows of a sequence count, and the rows may be slices of a wider tensor (any token stride that is a
+    sequence b in row cu_seqlens[b] + t (bfloat16 and int8 pools); a query length beyond the cu_seqlens[b + 1] -
+    cu_seqlens[b] rows of a sequence counts as their number, and the rows may be slices of a wider tensor (any token stride that is a
     multiple of 8 elements).
 
     Returns None: the pool tensors are the outputs, aliased to the inputs as the reference's cache tensors are
@@ -670,11 +701,13 @@ def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens,
         _need_device(n, t)
     _check(k_cache.dim() == 4, "k_cache must be [num_blocks, block_size, Hkv, D]")
     _check(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, "v_cache must match k_cache")
-    _check(k_cache.dtype in _DTYPE_CODE, f"unsupported pool dtype {k_cache.dtype}")
+    if k_cache.dtype not in _DTYPE_CODE:
+        raise ValueError(f"unsupported pool dtype {k_cache.dtype}")
     kv_dtype = _DTYPE_CODE[k_cache.dtype]
     _check(block_tables.dim() == 2 and block_tables.dtype == torch.int32, "block_tables must be int32 [B, max_blocks]")
     if packed:
-        _check(kv_dtype in (BF16, I8), f"packed rows go into bfloat16 or int8 pools (a float8 pool's scales belong to whole blocks), got {k_cache.dtype}")
+        if kv_dtype not in (BF16, I8):
+            raise ValueError(f"packed rows go into bfloat16 or int8 pools (a float8 pool's scales belong to whole blocks), got {k_cache.dtype}")
         strides = _token_rows("k_new", k_new), _token_rows("v_new", v_new)
         B = block_tables.shape[0]
         _check_cu("cu_seqlens", cu_seqlens, B)
@@ -683,10 +716,12 @@ def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens,
         _check(k_new.dim() == 4, "k_new must be [B, T, Hkv, D]")
         B, T, Hkv, D = k_new.shape
         want = torch.float32 if kv_dtype == F32 else torch.bfloat16
-        _check(k_new.dtype == want, f"k_new must be {want} for a {k_cache.dtype} pool, got {k_new.dtype}")
+        if k_new.dtype != want:
+            raise ValueError(f"k_new must be {want} for a {k_cache.dtype} pool, got {k_new.dtype}")
     _check(v_new.shape == k_new.shape and v_new.dtype == k_new.dtype, "v_new must match k_new")
     num_blocks, block_size = k_cache.shape[:2]
-    _check(tuple(k_cache.shape[2:]) == (Hkv, D), f"pool rows are {tuple(k_cache.shape[2:])}, new rows {(Hkv, D)}")
+    if tuple(k_cache.shape[2:]) != (Hkv, D):
+        raise ValueError(f"pool rows are {tuple(k_cache.shape[2:])}, new rows {(Hkv, D)}")
     _check(block_tables.shape[0] == B, "block_tables must be int32 [B, max_blocks]")
     _check(seq_lens.shape == (B,) and seq_lens.dtype == torch.int32, "seq_lens must be int32 [B]")
     _check(query_lens.shape == (B,) and query_lens.dtype == torch.int32, "query_lens must be int32 [B]")
@@ -694,7 +729,8 @@ def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens,
         _check_scales(kv_dtype, k_scale, v_scale, num_blocks, block_size, Hkv, "pool")
     else:
         _check(k_scale is None and v_scale is None, "k_scale / v_scale are for float8 and int8 pools only")
-    _check(kv_dtype != I8 and not packed or D in (32, 64, 128, 256), f"int8 pools and packed rows need head_dim 32, 64, 128 or 256 (got {D})")
+    if not (kv_dtype != I8 and not packed or D in (32, 64, 128, 256)):
+        raise ValueError(f"int8 pools and packed rows need head_dim 32, 64, 128 or 256 (got {D})")
     _same_device(k_new, v_new=v_new, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables,
                  seq_lens=seq_lens, query_lens=query_lens, k_scale=k_scale, v_scale=v_scale, cu_seqlens=cu_seqlens)
     with _on(k_new.device):
@@ -740,21 +776,24 @@ def read_kv(k_cache, v_cache, block_tables, seq_lens, cu_seqlens, total_tokens=N
         _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, "pool")
     else:
         _check(not scaled, "k_scale / v_scale are for float8 and int8 pools only")
-    _check(D % 8 == 0, f"head_dim {D} must be a multiple of 8")
+    if D % 8 != 0:
+        raise ValueError(f"head_dim {D} must be a multiple of 8")
     _check_cu("cu_seqlens", cu_seqlens, B)
     if out is None:
         _check(total_tokens is not None, "total_tokens (rows of the results) is needed without out")
         N = int(total_tokens)
-        _check(N >= 0, f"total_tokens {N} is negative")
+        if N < 0:
+            raise ValueError(f"total_tokens {N} is negative")
         out = tuple(torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
     else:
         _check(isinstance(out, (tuple, list)) and len(out) == 2, "out must be the pair (k, v)")
         for n, t in (("out[0]", out[0]), ("out[1]", out[1])):
             _need_device(n, t)
-            _check(t.dim() == 3 and tuple(t.shape[1:]) == (Hkv, D) and t.dtype == torch.bfloat16 and t.shape[0] == out[0].shape[0],
-                   f"{n} must be bfloat16 [tokens, {Hkv}, {D}]")
+            if not (t.dim() == 3 and tuple(t.shape[1:]) == (Hkv, D) and t.dtype == torch.bfloat16 and t.shape[0] == out[0].shape[0]):
+                raise ValueError(f"{n} must be bfloat16 [tokens, {Hkv}, {D}]")
         N = out[0].shape[0]
-        _check(total_tokens is None or int(total_tokens) == N, f"out has {N} rows, total_tokens says {total_tokens}")
+        if not (total_tokens is None or int(total_tokens) == N):
+            raise ValueError(f"out has {N} rows, total_tokens says {total_tokens}")
     _same_device(k_cache, v_cache=v_cache, block_tables=block_tables, seq_lens=seq_lens, cu_seqlens=cu_seqlens,
                  k_scale=k_scale, v_scale=v_scale, k=out[0], v=out[1])
     with _on(k_cache.device):

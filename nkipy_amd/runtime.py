@@ -27,7 +27,7 @@ from . import _lib, paged_attn
 
 _TENSOR_PARAMS = {"x", "o_weight", "bias", "q", "k_cache", "v_cache", "block_tables", "seq_lens", "query_lens", "k", "v",
                   "k_scale", "v_scale", "k_new", "v_new", "xq", "xk", "xv", "rope_cos", "rope_sin",
-                  "q_norm_weight", "k_norm_weight", "sinks"}
+                  "q_norm_weight", "k_norm_weight", "sinks", "cu_seqlens", "cu_seqlens_k"}
 ALIAS_SUFFIX = ".must_alias_input"      # nkipy/src/nkipy/core/trace.py:222
 # parameters an op writes in place (when given): they travel under the aliasing names
 _MUTATED = {"kv_write": ("k_cache", "v_cache", "k_scale", "v_scale"),
@@ -82,7 +82,7 @@ class DeviceKernel:
     _OPS = {"decode": paged_attn.decode, "prefill": paged_attn.prefill,
             "blocksparse_prefill": paged_attn.blocksparse_prefill,
             "kv_write": paged_attn.kv_write, "qk_norm_rope_kv_write": paged_attn.qk_norm_rope_kv_write,
-            "o_proj": paged_attn.o_proj}
+            "o_proj": paged_attn.o_proj, "packed_prefill": paged_attn.packed_prefill}
 
     def __init__(self, fn, name, signature, static_kwargs):
         self.fn, self.name = fn, name
@@ -107,8 +107,8 @@ class DeviceKernel:
 
     @classmethod
     def compile_and_load(cls, fn, name: str | None = None, **example_args) -> "DeviceKernel":
-        """fn: one of nkipy_amd.decode / prefill / blocksparse_prefill / kv_write /
-        qk_norm_rope_kv_write (or its name).  Tensor arguments (DeviceTensor or torch tensor), given
+        """fn: one of nkipy_amd.decode / prefill / blocksparse_prefill / packed_prefill / kv_write /
+        qk_norm_rope_kv_write / o_proj (or its name).  Tensor arguments (DeviceTensor or torch tensor), given
         under the op's parameter names, fix the expected shapes and dtypes; every other keyword
         (scale, partition_size, ...) becomes a static argument of the kernel."""
         if isinstance(fn, str):

@@ -13,9 +13,11 @@ the caller-allocates rule of nkipy/src/nkipy/runtime/device_tensor.py:51-74 carr
 captured graph replays without allocations.  Optional tensors may be None; `sliding_window` 0 means
 none.
 
-`workspace` (paged_decode, paged_prefill, o_proj): optional uint8 scratch for split-K partials, sized with
+The operators named *_fp8 take the int8 pools too (k_scale / v_scale then [num_blocks, Hkv, block_size]).
+
+`workspace` (paged_decode, paged_prefill, packed_prefill, o_proj): optional uint8 scratch for split-K partials, sized with
 `paged_attn.decode_workspace_bytes` / `lib.pa_verify_workspace_bytes` / `pa_prefill_workspace_bytes` /
-`o_proj_workspace_bytes`.  Without it the ops use a buffer cached per (device, stream), which all graphs
+`packed_prefill_workspace_bytes` / `o_proj_workspace_bytes`.  Without it the ops use a buffer cached per (device, stream), which all graphs
 captured on one stream share.  A caller that replays several graphs at once gives each its own.  The
 scratch carries nothing from call to call, so it is not declared as a mutated argument.
 """
@@ -217,6 +219,33 @@ def verify_step_fp8(xq: torch.Tensor, xk: torch.Tensor, xv: torch.Tensor, k_cach
                            sliding_window=_win(sliding_window))
 
 
+# int8 pools (a scale per token and kv head): the write, and reading the pool back as dense rows
+@torch.library.custom_op(f"{_NS}::paged_kv_write_int8", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"), device_types="cuda")
+def paged_kv_write_int8(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                        k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                        query_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None) -> None:
+    paged_attn.kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens, k_scale=k_scale, v_scale=v_scale,
+                        cu_seqlens=cu_seqlens)
+
+
+@torch.library.custom_op(f"{_NS}::read_kv", mutates_args=("k_out", "v_out"), device_types="cuda")
+def read_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+            cu_seqlens: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+            v_scale: Optional[torch.Tensor] = None) -> None:
+    paged_attn.read_kv(k_cache, v_cache, block_tables, seq_lens, cu_seqlens, k_scale=k_scale, v_scale=v_scale, out=(k_out, v_out))
+
+
+# whole prompts of different lengths, packed row behind row (examples/models/qwen3/kernels/attention.py:112-144 per sequence)
+@torch.library.custom_op(f"{_NS}::packed_prefill", mutates_args=("out",), device_types="cuda")
+def packed_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float, out: torch.Tensor,
+                   cu_seqlens_k: Optional[torch.Tensor] = None, query_lens: Optional[torch.Tensor] = None,
+                   seq_lens: Optional[torch.Tensor] = None, max_seq_len: int = 0, sinks: Optional[torch.Tensor] = None,
+                   sliding_window: int = 0, workspace: Optional[torch.Tensor] = None) -> None:
+    paged_attn.packed_prefill(q, k, v, cu_seqlens, scale, cu_seqlens_k=cu_seqlens_k, query_lens=query_lens, seq_lens=seq_lens,
+                              max_seq_len=max_seq_len or None, sinks=sinks, sliding_window=_win(sliding_window), out=out,
+                              workspace=workspace)
+
+
 def _no_cpu(name):
     def impl(*args, **kwargs):
         raise NotImplementedError(f"{_NS}::{name} runs hand-written HIP kernels and has no CPU path; "
@@ -230,10 +259,11 @@ for _op, _name in ((paged_decode, "paged_decode"), (paged_prefill, "paged_prefil
                    (qk_norm_rope_kv_write_fp8, "qk_norm_rope_kv_write_fp8"),
                    (k_norm_rope_kv_write, "k_norm_rope_kv_write"), (k_norm_rope_kv_write_fp8, "k_norm_rope_kv_write_fp8"),
                    (o_proj, "o_proj"), (decode_step, "decode_step"), (decode_step_fp8, "decode_step_fp8"),
-                   (verify_step, "verify_step"), (verify_step_fp8, "verify_step_fp8")):
+                   (verify_step, "verify_step"), (verify_step_fp8, "verify_step_fp8"),
+                   (paged_kv_write_int8, "paged_kv_write_int8"), (read_kv, "read_kv"), (packed_prefill, "packed_prefill")):
     _op.register_kernel("cpu")(_no_cpu(_name))
     _op.register_fake(lambda *args, **kwargs: None)      # outputs are caller-allocated: nothing to infer
 
 OPS = ("paged_decode", "paged_prefill", "blocksparse_prefill", "paged_kv_write", "paged_kv_write_fp8",
        "qk_norm_rope_kv_write", "qk_norm_rope_kv_write_fp8", "k_norm_rope_kv_write", "k_norm_rope_kv_write_fp8", "o_proj",
-       "decode_step", "decode_step_fp8", "verify_step", "verify_step_fp8")
+       "decode_step", "decode_step_fp8", "verify_step", "verify_step_fp8", "paged_kv_write_int8", "read_kv", "packed_prefill")

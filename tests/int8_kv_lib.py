@@ -90,13 +90,15 @@ def attention64(q, k, v, scale, first, window=0, sinks=None):
     return out, mag, reach
 
 
-def attention_tolerance(out, mag, reach, D, q_rounded=False):
+def attention_tolerance(out, mag, reach, D):
     """What the kernels may be off by, element by element.  The probabilities (times the value's scale) are rounded to bf16
     once, at most H relative each: H * sum p |v|.  The result is rounded once: H |out|.  Scores are float32 sums of D
     products (and of the scale and the reference): an absolute error of at most (D + 8) 2^-24 reach, which moves a
     probability and the sum it is divided by by twice that, relatively; exp2 itself and the sums over the keys stay
-    within 2^-18.  q_rounded: the query is rounded once more after the scale has gone into it (H reach on every score)."""
-    score = (D + 8) * 2.0 ** -24 * reach + (H * reach if q_rounded else 0.0)
+    within 2^-18.  (Over an int8 pool the probabilities are rounded to 16 bits and the query's elements to 2^-16 of the
+    row's largest, which is below what the 8 bits of the other kernels allow: 2^-16 q_max sum |k| scale <= 2^-8 of the
+    room H * sum p |v| leaves as long as the scores stay below a few hundred.)"""
+    score = (D + 8) * 2.0 ** -24 * reach
     grow = np.expm1(min(2 * score, 1.0))
     return (H + grow + 2.0 ** -18) * mag * (1 + H) + H * np.abs(out) + 1e-30
 

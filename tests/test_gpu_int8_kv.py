@@ -228,6 +228,41 @@ def _decode_case(pa, rng, ctxs, Hq, Hkv, D, bs, T=1, qlens=None, window=None, wi
     return got
 
 
+@pytest.mark.parametrize("bound", [64, 700, 1024, 2500])
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (16, 4, 64), (12, 1, 128)])
+def test_decode_with_a_bound(pa, rng, Hq, Hkv, D, bound):
+    """The kernels a length bound chooses: one partition on eight waves, several, the balanced schedule."""
+    _decode_case(pa, rng, [1, 0, 31, bound, bound // 2 + 1, 33], Hq, Hkv, D, 64, bound=bound)
+
+
+def test_refusals(pa):
+    t = lambda *s, dt=torch.int8: torch.zeros(s, dtype=dt, device="cuda")              # noqa: E731
+    kc, sc = t(4, 16, 2, 64), t(4, 2, 16, dt=torch.float32)
+    tb, ln = t(1, 4, dt=torch.int32), t(1, dt=torch.int32)
+    q, x = t(1, 4, 64, dt=torch.bfloat16), t(1, 3, 2, 64, dt=torch.bfloat16)
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    fp8_scale = t(4, 2, dt=torch.float32)
+    pa.decode(q, kc, kc, tb, ln, 0.1, k_scale=sc, v_scale=sc)
+    for kw in [{}, {"k_scale": sc}, {"k_scale": fp8_scale, "v_scale": fp8_scale}, {"k_scale": sc.double(), "v_scale": sc.double()}]:
+        for call in (lambda **k: pa.decode(q, kc, kc, tb, ln, 0.1, **k), lambda **k: pa.kv_write(x, x, kc, kc, tb, ln, ln, **k),
+                     lambda **k: pa.read_kv(kc, kc, tb, ln, cu, 3, **k), lambda **k: pa.verify(x.repeat(1, 1, 2, 1), kc, kc, tb, ln, ln, 0.1, **k)):
+            with pytest.raises(ValueError):
+                call(**kw)
+    s = {"k_scale": sc, "v_scale": sc}
+    long = t(1, 65, 4, 64, dt=torch.bfloat16)
+    odd = t(4, 24, 2, 64)
+    odd_s = t(4, 2, 24, dt=torch.float32)
+    for call in (lambda: pa.prefill(long, kc, kc, tb, ln, ln, 0.1, **s), lambda: pa.prefill(long[:, :4].contiguous(), kc, kc, tb, ln, ln, 0.1, route="tiled", **s),
+                 lambda: pa.decode(q, odd, odd, tb, ln, 0.1, k_scale=odd_s, v_scale=odd_s), lambda: pa.decode(q.float(), kc, kc, tb, ln, 0.1, **s),
+                 lambda: pa.read_kv(kc, kc, tb, ln, cu, **s), lambda: pa.read_kv(kc, kc, tb, ln, cu, -1, **s), lambda: pa.read_kv(kc, kc, tb, ln, cu.long(), 3, **s),
+                 lambda: pa.read_kv(kc, kc, tb, ln, cu, 3, out=(x[0], x[0].float()), **s), lambda: pa.read_kv(kc, kc, tb, ln, cu, 4, out=(x[0], x[0]), **s),
+                 lambda: pa.read_kv(kc.float(), kc.float(), tb, ln, cu, 3), lambda: pa.kv_write(x, x, kc, kc, tb, ln, ln, cu_seqlens=cu, **s),
+                 lambda: pa.kv_write(x[0], x[0], kc, kc, tb, ln, ln, cu_seqlens=cu[:1], **s),
+                 lambda: pa.kv_write(x[0], x[0], kc.view(torch.float8_e4m3fn), kc.view(torch.float8_e4m3fn), tb, ln, ln, cu_seqlens=cu, k_scale=fp8_scale, v_scale=fp8_scale)):
+        with pytest.raises(ValueError):
+            call()
+
+
 @pytest.mark.parametrize("impl", [0, 2, 3])
 @pytest.mark.parametrize("Hq,Hkv,D,bs", [(32, 8, 128, 32), (8, 8, 64, 16), (40, 2, 128, 16), (7, 1, 64, 64), (6, 3, 128, 128)])
 def test_decode(pa, rng, debug_switch, Hq, Hkv, D, bs, impl):
