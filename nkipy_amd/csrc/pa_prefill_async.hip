@@ -603,7 +603,9 @@ void prefill_async_kernel(PrefillParams p) {
       stage_i = stage_i + 1 == NST ? 0 : stage_i + 1;
       return;
     }
-    issue_tile(w_i.kt < ntiles ? w_i.kt : kt_first, stage_i);
+    // (two stages: the loop waits for all copies anyway, so nothing has to be requested past the end -- where a workgroup
+    // walks two or three tiles the repeated one was a third of its copies, waited for in the end)
+    if (!PACKED || NST > 2 || w_i.kt < ntiles) issue_tile(w_i.kt < ntiles ? w_i.kt : kt_first, stage_i);
     if (FP8) {
       const long si = (long)min(max(blk_pf[0], 0), p.num_blocks - 1) * p.Hkv + kv0;
       ksq[3] = ((const_f32_ptr)(uintptr_t)p.k_scale)[si];
