@@ -46,6 +46,30 @@ def _need_device(name, t):
         raise ValueError(f"{name} must be contiguous")
 
 
+def _all_on(ref, needed, optional=()):
+    """Every (name, tensor) of `needed`, and those of `optional` that are not None, is a contiguous tensor on ref's device:
+    `_need_device` and `_same_device` of all of them in one pass, for the calls that a decode loop issues by the thousand."""
+    try:
+        idx = ref.get_device()
+        for _, t in needed:
+            if not (t.is_cuda and t.is_contiguous() and t.get_device() == idx):
+                break
+        else:
+            for _, t in optional:
+                if t is not None and not (t.is_cuda and t.is_contiguous() and t.get_device() == idx):
+                    break
+            else:
+                return
+    except AttributeError:                   # something that is not a tensor: named below
+        pass
+    named = tuple(needed) + tuple((n, t) for n, t in optional if t is not None)
+    for n, t in named:
+        _need_device(n, t)
+    for n, t in named:
+        if t.get_device() != ref.get_device():
+            raise ValueError(f"{n} is on {t.device}, expected {ref.device}")
+
+
 def _check(cond, msg):
     # (the calls a decode loop issues by the thousand spell the raise out where the text is formatted: an argument is
     # formatted whether it is needed or not, and a dozen of them were a quarter of a small call's host time)
@@ -116,7 +140,7 @@ def _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, what="
         raise ValueError(f"{'fp8' if kv_code == FP8 else 'int8'} {what} needs both k_scale and v_scale")
     for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
         _need_device(n, t)
-        if not (t.dtype == torch.float32 and t.shape == shape):
+        if t.dtype != torch.float32 or t.shape != shape:
             raise ValueError(f"{n} must be float32 {text}")
 
 
@@ -182,7 +206,7 @@ def _workspace(device, nbytes, stream=None):
     graphs concurrently pass a `workspace=` of their own per graph, sized with the *_workspace_bytes functions,
     and keep it alive."""
     key = (device, (stream or _stream_ptr(device)).value)
-    if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+    if (device.type if isinstance(device, torch.device) else torch.device(device).type) == "cuda" and torch.cuda.is_current_stream_capturing():
         buf = _graph_workspaces.get(key)
         if buf is None or buf.numel() < nbytes:
             if buf is not None:
@@ -269,9 +293,8 @@ def decode(q, k_cache, v_cache, block_tables, seq_lens, scale, *, k_scale=None, 
     q_transform: a `QTransform`; q then holds the rows before norm and rotation (same shapes).
     """
     lib = _lib.load()
-    for n, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache),
-                 ("block_tables", block_tables), ("seq_lens", seq_lens)):
-        _need_device(n, t)
+    _all_on(q, (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens)),
+            (("k_scale", k_scale), ("v_scale", v_scale), ("out", out)))
     _check(q.dim() == 3, "q must be [B, Hq, D]")
     B, Hq, D = q.shape
     if q.dtype not in (torch.float32, torch.bfloat16):
@@ -303,14 +326,11 @@ def decode(q, k_cache, v_cache, block_tables, seq_lens, scale, *, k_scale=None, 
     msl = cap if max_seq_len is None else int(max_seq_len)
     if not (0 < msl <= cap):
         raise ValueError(f"max_seq_len {msl} outside (0, {cap}]")
-    _same_device(q, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables, seq_lens=seq_lens,
-                 k_scale=k_scale, v_scale=v_scale, out=out)
     if validate_tables:
         check_block_tables(block_tables, seq_lens, num_blocks, block_size)
     if out is None:
         out = torch.empty_like(q)
     else:
-        _need_device("out", out)
         _check(out.shape == q.shape and out.dtype == q.dtype, "out must match q in shape and dtype")
     qt_keep, qt_ptr = _qt_arg(q_transform, D, q)
     with _on(q.device):
@@ -407,9 +427,8 @@ def prefill(q, k_cache, v_cache, block_tables, seq_lens, query_lens, scale, *, k
     length cached in front of it (max_seq_len < 3 T) runs unsplit, which is faster there.
     """
     lib = _lib.load()
-    for n, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables),
-                 ("seq_lens", seq_lens), ("query_lens", query_lens)):
-        _need_device(n, t)
+    _all_on(q, (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens),
+                ("query_lens", query_lens)), (("k_scale", k_scale), ("v_scale", v_scale), ("out", out)))
     _check(q.dim() == 4, "q must be [B, T, Hq, D]")
     B, T, Hq, D = q.shape
     _check(q.dtype == torch.bfloat16, "prefill supports bfloat16 only")
@@ -443,14 +462,11 @@ def prefill(q, k_cache, v_cache, block_tables, seq_lens, query_lens, scale, *, k
         if not (can_verify):
             raise ValueError(f"the verify kernel needs T <= 64, head_dim 64 or 128 and a power-of-two block size >= 16 "
                              f"(T={T}, D={D}, block_size={block_size})")
-    _same_device(q, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables, seq_lens=seq_lens,
-                 query_lens=query_lens, k_scale=k_scale, v_scale=v_scale, out=out)
     if validate_tables:
         check_block_tables(block_tables, seq_lens, num_blocks, block_size)
     if out is None:
         out = torch.empty_like(q)
     else:
-        _need_device("out", out)
         _check(out.shape == q.shape and out.dtype == q.dtype, "out must match q in shape and dtype")
     qt_keep, qt_ptr = _qt_arg(q_transform, D, q)
     stream = _stream_ptr(q.device)
@@ -566,7 +582,8 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
         raise ValueError(f"Hq={Hq} is not a multiple of Hkv={Hkv}")
     if D not in (64, 128):
         raise ValueError(f"head_dim {D} must be 64 or 128")
-    _need_device("cu_seqlens", cu_seqlens)
+    _all_on(q, (("cu_seqlens", cu_seqlens),), (("cu_seqlens_k", cu_seqlens_k), ("query_lens", query_lens), ("seq_lens", seq_lens), ("out", out)))
+    _same_device(q, k=k, v=v)
     _check(cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1, "cu_seqlens must be int32 [num_seqs + 1]")
     S = cu_seqlens.shape[0] - 1
     _check_cu("cu_seqlens", cu_seqlens, S)
@@ -578,7 +595,6 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
         _check_cu("cu_seqlens_k", cu_seqlens_k, S)
     for n, t in (("query_lens", query_lens), ("seq_lens", seq_lens)):
         if t is not None:
-            _need_device(n, t)
             if not (t.shape == (S,) and t.dtype == torch.int32):
                 raise ValueError(f"{n} must be int32 [num_seqs]")
     if not (max_seq_len is None or int(max_seq_len) > 0):
@@ -591,7 +607,6 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
         _need_device("out", out)
         if not (tuple(out.shape) == (Nq, Hq, D) and out.dtype == torch.bfloat16):
             raise ValueError(f"out must be bfloat16 {(Nq, Hq, D)}")
-    _same_device(q, k=k, v=v, cu_seqlens=cu_seqlens, cu_seqlens_k=cu_seqlens_k, query_lens=query_lens, seq_lens=seq_lens, out=out)
     with _on(q.device):
         stream = _stream_ptr(q.device)
         key = (S, Nq, Nk, Hq, Hkv, D, bound)
@@ -646,22 +661,27 @@ def gather_kv(cache, block_tables, seq_lens, max_seq_len=None):
 def _token_rows(name, t, dtype=torch.bfloat16):
     """Packed rows [tokens, heads, D] on the device whose tokens may lie apart (a slice of a wider projection output): the
     heads and their elements are adjacent, and the token stride is a multiple of 8 elements.  Returns the token stride."""
-    if isinstance(t, torch.Tensor) and t.is_cuda and not t.is_contiguous():
-        if t.dim() != 3:
-            raise ValueError(f"{name} must be [tokens, heads, D]")
-        if not ((t.stride(2) == 1 or t.shape[2] == 1) and (t.stride(1) == t.shape[2] or t.shape[1] == 1)):
-            raise ValueError(f"{name}: the heads of a token must be adjacent rows of D elements (strides {t.stride()})")
-        if not (t.stride(0) % 8 == 0 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1] * t.shape[2])):
-            raise ValueError(f"{name}: the token stride {t.stride(0)} must be a multiple of 8 elements and at least a token's row")
-    else:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
         _need_device(name, t)
-        if t.dim() != 3:
-            raise ValueError(f"{name} must be [tokens, heads, D]")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, D]")
+    n, heads, D = t.shape
+    row = heads * D
+    if t.is_contiguous():
+        step = row
+    else:
+        step, across, along = t.stride()
+        if (along != 1 and D != 1) or (across != D and heads != 1):
+            raise ValueError(f"{name}: the heads of a token must be adjacent rows of D elements (strides {t.stride()})")
+        if n <= 1:
+            step = row
+        elif step % 8 != 0 or step < row:
+            raise ValueError(f"{name}: the token stride {step} must be a multiple of 8 elements and at least a token's row")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.data_ptr() % 16 != 0:
         raise ValueError(f"{name} must start on a 16-byte boundary")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return step
 
 
 def _check_cu(name, cu, n):
@@ -695,10 +715,9 @@ def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens,
     """
     lib = _lib.load()
     packed = cu_seqlens is not None
-    for n, t in (() if packed else (("k_new", k_new), ("v_new", v_new))) + \
-                (("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens),
-                 ("query_lens", query_lens)):
-        _need_device(n, t)
+    _all_on(k_cache, (("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens),
+                      ("query_lens", query_lens)) + (() if packed else (("k_new", k_new), ("v_new", v_new))),
+            (("k_scale", k_scale), ("v_scale", v_scale), ("cu_seqlens", cu_seqlens)))
     _check(k_cache.dim() == 4, "k_cache must be [num_blocks, block_size, Hkv, D]")
     _check(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, "v_cache must match k_cache")
     if k_cache.dtype not in _DTYPE_CODE:
@@ -731,8 +750,8 @@ def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens,
         _check(k_scale is None and v_scale is None, "k_scale / v_scale are for float8 and int8 pools only")
     if not (kv_dtype != I8 and not packed or D in (32, 64, 128, 256)):
         raise ValueError(f"int8 pools and packed rows need head_dim 32, 64, 128 or 256 (got {D})")
-    _same_device(k_new, v_new=v_new, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables,
-                 seq_lens=seq_lens, query_lens=query_lens, k_scale=k_scale, v_scale=v_scale, cu_seqlens=cu_seqlens)
+    if packed:
+        _same_device(k_cache, k_new=k_new, v_new=v_new)
     with _on(k_new.device):
         if packed:
             rc = lib.pa_kv_write_packed(_ptr(k_new), _ptr(v_new), *strides, _ptr(cu_seqlens), k_new.shape[0], _ptr(k_cache),
@@ -763,8 +782,9 @@ def read_kv(k_cache, v_cache, block_tables, seq_lens, cu_seqlens, total_tokens=N
     memory held.
     """
     lib = _lib.load()
-    for n, t in (("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens)):
-        _need_device(n, t)
+    out0, out1 = (None, None) if not isinstance(out, (tuple, list)) or len(out) != 2 else out
+    _all_on(k_cache, (("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens),
+                      ("cu_seqlens", cu_seqlens)), (("k_scale", k_scale), ("v_scale", v_scale), ("out[0]", out0), ("out[1]", out1)))
     _check(block_tables.dim() == 2, "block_tables must be int32 [B, max_blocks_per_seq]")
     B = block_tables.shape[0]
     _check_paging(k_cache, v_cache, block_tables, seq_lens, B)
@@ -784,24 +804,22 @@ def read_kv(k_cache, v_cache, block_tables, seq_lens, cu_seqlens, total_tokens=N
         N = int(total_tokens)
         if N < 0:
             raise ValueError(f"total_tokens {N} is negative")
-        out = tuple(torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
+        out0 = torch.empty((N, Hkv, D), dtype=torch.bfloat16, device=k_cache.device)
+        out1 = torch.empty_like(out0)
     else:
-        _check(isinstance(out, (tuple, list)) and len(out) == 2, "out must be the pair (k, v)")
-        for n, t in (("out[0]", out[0]), ("out[1]", out[1])):
-            _need_device(n, t)
-            if not (t.dim() == 3 and tuple(t.shape[1:]) == (Hkv, D) and t.dtype == torch.bfloat16 and t.shape[0] == out[0].shape[0]):
+        _check(out0 is not None and out1 is not None, "out must be the pair (k, v)")
+        for n, t in (("out[0]", out0), ("out[1]", out1)):
+            if not (t.dim() == 3 and tuple(t.shape[1:]) == (Hkv, D) and t.dtype == torch.bfloat16 and t.shape[0] == out0.shape[0]):
                 raise ValueError(f"{n} must be bfloat16 [tokens, {Hkv}, {D}]")
-        N = out[0].shape[0]
+        N = out0.shape[0]
         if not (total_tokens is None or int(total_tokens) == N):
             raise ValueError(f"out has {N} rows, total_tokens says {total_tokens}")
-    _same_device(k_cache, v_cache=v_cache, block_tables=block_tables, seq_lens=seq_lens, cu_seqlens=cu_seqlens,
-                 k_scale=k_scale, v_scale=v_scale, k=out[0], v=out[1])
     with _on(k_cache.device):
         rc = lib.pa_read_kv(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_tables), _ptr(seq_lens),
-                            _ptr(cu_seqlens), _ptr(out[0]), _ptr(out[1]), N, B, Hkv, D, block_size, block_tables.shape[1],
+                            _ptr(cu_seqlens), _ptr(out0), _ptr(out1), N, B, Hkv, D, block_size, block_tables.shape[1],
                             num_blocks, kv_code, _stream_ptr(k_cache.device))
     _raise_on(rc, "pa_read_kv")
-    return out[0], out[1]
+    return out0, out1
 
 
 def rope_tables(head_dim: int, max_seq_len: int, base: float = 10000.0, device="cuda"):
