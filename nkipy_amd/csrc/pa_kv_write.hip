@@ -561,11 +561,15 @@ hipError_t launch_rows_kind(const KvWriteParams& p, hipStream_t s) {
 }
 
 template <int CPR>
-void launch_xform(const KvWriteParams& p, dim3 grid, hipStream_t s) {
+hipError_t launch_xform(const KvWriteParams& p, dim3 grid, hipStream_t s) {
   if (p.q_in) hipLaunchKernelGGL((q_norm_rope_kernel<CPR, QWG, QUNR>), dim3(p.T, p.B), dim3(QWG), 0, s, p);
-  if (p.kv_dtype == PA_INT8) { (void)launch_rows<1, CPR>(p, s); return; }
+  if (p.kv_dtype == PA_INT8) {
+    const hipError_t q_error = hipGetLastError();        // (the Q rows' launch)
+    return q_error != hipSuccess ? q_error : launch_rows<1, CPR>(p, s);
+  }
   if (p.kv_dtype == PA_FP8_E4M3FN) hipLaunchKernelGGL((kv_write_kernel<1, CPR>), grid, dim3(WG), 0, s, p);
   else hipLaunchKernelGGL((kv_write_kernel<2, CPR>), grid, dim3(WG), 0, s, p);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -578,11 +582,9 @@ hipError_t launch_kv_write(const KvWriteParams& p, hipStream_t s) {
   const int touched = (p.T + p.block_size - 1) / p.block_size + 1;   // a chunk of T rows spans at most this many blocks
   const dim3 grid(2 * touched, p.Hkv, p.B);
   if (p.rope_cos != nullptr) {
-    if (p.D == 64) launch_xform<8>(p, grid, s);
-    else if (p.D == 128) launch_xform<16>(p, grid, s);
-    else if (p.D == 256) launch_xform<32>(p, grid, s);
-    else return hipErrorInvalidValue;
-    return hipGetLastError();
+    if (p.D == 64) return launch_xform<8>(p, grid, s);
+    if (p.D == 128) return launch_xform<16>(p, grid, s);
+    return p.D == 256 ? launch_xform<32>(p, grid, s) : hipErrorInvalidValue;
   }
   if (p.kv_dtype == PA_INT8) return launch_rows_kind<1>(p, s);
   if (p.cu) return p.kv_dtype == PA_BF16 ? launch_rows_kind<2>(p, s) : hipErrorInvalidValue;

@@ -181,7 +181,7 @@ __device__ __forceinline__ PackedTile packed_tile(const PrefillParams& p, int x,
     r.tq = min(max(p.query_lens ? p.query_lens[r.b] : r.seg, 0), max(r.seg, 0));
     r.ctx = min(max(p.seq_lens ? p.seq_lens[r.b] : r.seg_k, 0), r.seg_k);
     r.tiles = r.seg > 0 ? (r.seg * mult + (1 << shift) - 1) >> shift : 0;
-    r.tile = r.tile >= r.tiles ? -1 : r.tiles - 1 - r.tile;
+    r.tile = r.tile < 0 || r.tile >= r.tiles ? -1 : r.tiles - 1 - r.tile;
     return r;
   }
   return p.B <= 64 ? packed_tile_ranked<1>(p, x, shift, mult, lane) : packed_tile_ranked<8>(p, x, shift, mult, lane);

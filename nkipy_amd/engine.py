@@ -273,7 +273,9 @@ class PagedAttention:
     (`packed_prefill`).  Returns [max_seqs, T, Hq, D] (a preallocated buffer, overwritten by the next step of
     the same T), or, when the layer was given `o_weight`, the output projection of it, [max_seqs, T, hidden].
 
-    `attend` makes no host synchronisation and, after the first call of a given T, no allocation, so the
+    `attend` makes no host synchronisation and, after the first call of a given T, no allocation (but for the rows that a
+    long chunk over an int8 cache reads back: those of the contexts that take part, or captured into a graph max_seqs
+    times the length bound), so the
     launch-bound decode step of a stack of layers can be captured into one HIP graph (`torch.cuda.graph`) with
     xq / xk / xv as static buffers and replayed every step: `begin_step` stays outside the graph (it publishes
     the step's table rows and lengths, which the replayed kernels read from the same device tensors).  A captured

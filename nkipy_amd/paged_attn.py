@@ -569,7 +569,8 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
     other keys are never read.  A query that sees no key gets zeros; rows that belong to no sequence are left as they
     are (whatever the memory held in a result allocated here).
     K and V rows are expected to be finite: a V row with an infinity or a NaN can reach the rows of up to 95
-    queries in front of it as well (their weight for it is 0, and 0 x inf is not).
+    queries in front of it as well, and of as many behind those whose window it is in (their weight for it is 0, and
+    0 x inf is not).
     max_seq_len: host-known upper bound of a sequence's keys; sizes the split of calls with few queries over many keys
     (default Nk).  sinks [Hq] / sliding_window as in `decode`, the window counted back from each query.
     """

@@ -202,10 +202,11 @@ def test_read_back_bit_exact(pa, rng, kind, D, bs, Hkv):
         assert torch.equal(fresh[0][a:z], want[0][a:z]) and torch.equal(fresh[1][a:z], want[1][a:z])
 
 
-def _decode_case(pa, rng, ctxs, Hq, Hkv, D, bs, T=1, qlens=None, window=None, with_sinks=False, bound=None, **kw):
+def _decode_case(pa, rng, ctxs, Hq, Hkv, D, bs, T=1, qlens=None, window=None, with_sinks=False, bound=None, size=1.0, **kw):
     pool = int8_pool(rng, ctxs, bs, Hkv, D, spread=0.5)
     B = len(ctxs)
-    q = O.round_to_bf16(rng.standard_normal((B, T, Hq, D)).astype(np.float32))
+    q = O.round_to_bf16(rng.standard_normal((B, T, Hq, D)).astype(np.float32)) * np.float32(size)
+    pool["ks"] /= np.float32(size)
     scale = 1.0 / np.sqrt(D)
     sinks = rng.standard_normal(Hq).astype(np.float32) if with_sinks else None
     args = (dev(pool["k"]), dev(pool["v"]), dev(pool["tables"]), dev(np.asarray(ctxs, np.int32)))
@@ -224,6 +225,12 @@ def _decode_case(pa, rng, ctxs, Hq, Hkv, D, bs, T=1, qlens=None, window=None, wi
         o, mag, reach = attention64(q[b, :n].astype(np.float64), context(pool, "k", b, c, bs), context(pool, "v", b, c, bs), scale,
                                     c - n, window or 0, sinks)
         want[b, :n], tol[b, :n] = o, attention_tolerance(o, mag, reach, D)
+        if size < 2.0 ** -105:
+            # A row's step is its largest element / 32 512, but not below 2^-120 (the step's reciprocal has to have one
+            # itself): every element may be off by 2^-121, a score by that times sum |k| scale, and a probability and the sum
+            # it is divided by by twice the score's error, relatively.
+            off = 2.0 ** -121 * np.abs(context(pool, "k", b, c, bs)).sum(-1).max() * scale
+            tol[b, :n] += np.expm1(2 * off) * mag
     assert_within(got, want, tol)
     return got
 
@@ -283,6 +290,26 @@ def test_decode_window_and_sinks(pa, rng, debug_switch, impl, window, D):
 def test_verify(pa, rng, Hq, Hkv, D, T, bound):
     qlens = [T, 1, 0, min(T, 2), T]
     _decode_case(pa, rng, [T, 500, 40, 1000, T + 31], Hq, Hkv, D, 32, T=T, qlens=qlens, bound=bound)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -118, 2.0 ** -110, 2.0 ** -103, 2.0 ** -60, 2.0 ** 60, 2.0 ** 114])
+def test_queries_of_any_size(pa, rng, size):
+    """A query's size cancels against the keys': sizes near either end of the type's range take the same way."""
+    _decode_case(pa, rng, [1, 33, 700], 8, 2, 128, 16, size=size)
+
+
+def test_the_largest_queries(pa, rng):
+    """An element near the type's largest number, on a channel where all keys are zero: all scores are zero."""
+    D, bs, c = 128, 16, 300
+    pool = int8_pool(rng, [c], bs, 2, D)
+    pool["k"][..., 5] = 0
+    q = np.zeros((1, 8, D), np.float32)
+    q[..., 5] = O.round_to_bf16(np.float32(3.3e38) * rng.uniform(0.26, 1.0, (1, 8)).astype(np.float32))
+    got = pa.decode(bf16(q), dev(pool["k"]), dev(pool["v"]), dev(pool["tables"]), dev(np.asarray([c], np.int32)), 0.1,
+                    k_scale=dev(pool["ks"]), v_scale=dev(pool["vs"]))
+    o, mag, reach = attention64(q.astype(np.float64), context(pool, "k", 0, c, bs), context(pool, "v", 0, c, bs), 0.1, c - 1)
+    assert reach == 0.0
+    assert_within(got, o, attention_tolerance(o, mag, reach, D))
 
 
 @pytest.mark.parametrize("rows", [16, 32])

@@ -246,6 +246,36 @@ def test_a_row_that_is_no_number_stays_alone(pa, rng, D):
     assert torch.equal(pa.packed_prefill(q, k, v, cu, 0.1)[:90], want[:90])
 
 
+def test_many_boundaries_that_lie(pa, rng):
+    """The same past the number of sequences that the ranking holds: a first boundary behind the first row, and one far out."""
+    n, S, D = 900, 700, 64
+    q, k, v = (bf16(rng.standard_normal((n, 2, D))) for _ in range(3))
+    cu = np.sort(rng.integers(300, n, S + 1)).astype(np.int32)
+    want = pa.packed_prefill(q, k, v, dev(cu), 0.1, out=torch.full_like(q, 3.0))
+    assert (want[:cu[0]] == 3).all() and (want[cu[-1]:] == 3).all()
+    for i in range(0, S, 97):
+        a, z = int(cu[i]), int(cu[i + 1])
+        one = pa.packed_prefill(q[a:z], k[a:z], v[a:z], dev(np.asarray([0, z - a], np.int32)), 0.1) if z > a else q[a:z]
+        assert torch.equal(want[a:z], one)
+    cu[[0, 350, 600]] = [-7, 2 ** 31 - 1, -2 ** 31]
+    assert torch.isfinite(pa.packed_prefill(q, k, v, dev(cu), 0.1, out=torch.zeros_like(q))).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 1, 128), (4, 2, 64)])
+def test_rows_past_32_bits(pa, rng, Hq, Hkv, D):
+    """Rows of a tensor of 5 GB, on both sides of 2^31 elements and bytes, against the same rows packed closely."""
+    stride, n = 1 << 16, 40000
+    wide = torch.empty((n, stride), dtype=torch.bfloat16, device="cuda")
+    dq, dk, dv = (wide[:, a:a + h * D].view(n, h, D) for a, h in ((0, Hq), (8192, Hkv), (16384, Hkv)))
+    q, k, v = (torch.randn((n, h, D), device="cuda").to(torch.bfloat16) for h in (Hq, Hkv, Hkv))
+    dq.copy_(q), dk.copy_(k), dv.copy_(v)
+    cu = dev(np.asarray([0, 100, 16300, 16500, 32700, 32900, 39800, n], np.int32))
+    lens = dev(np.asarray([100, 150, 200, 150, 200, 150, 200], np.int32))
+    for kw in ({}, {"sliding_window": 64}):
+        got = pa.packed_prefill(dq, dk, dv, cu, 0.1, query_lens=lens, seq_lens=lens, **kw)
+        assert torch.equal(got, pa.packed_prefill(q, k, v, cu, 0.1, query_lens=lens, seq_lens=lens, **kw))
+
+
 def test_empty_calls(pa):
     e = lambda n, h: torch.empty((n, h, 64), dtype=torch.bfloat16, device="cuda")      # noqa: E731
     i32 = lambda x: dev(np.asarray(x, np.int32))                                       # noqa: E731
