@@ -209,8 +209,17 @@ __device__ __forceinline__ PackedTile packed_tile(const PrefillParams& p, int x,
 // tokens for two adjacent q heads: every K and V tile then serves twice the matrix work (at head dim 64 a tile
 // otherwise has half the matrix work of head dim 128 against the same copies and barrier), and between two
 // barriers the waves of a SIMD have twice as many matrix and vector phases to slide under one another.
+// TT 1 (packed form, short prompts and narrow windows): 32-key tiles halve the stages, 32 KB of LDS per workgroup.  At head
+// dim 64 with one q head per wave the registers (120) leave room for four workgroups per CU as well.
+constexpr int prefill_waves_per_simd(int mode, int tt, int dh) { return mode == 2 && tt == 1 && dh == 64 ? 4 : 2; }
+constexpr int prefill_stages(bool sparse, int nw) { return nw == 8 ? (sparse ? 5 : 4) : 2; }
+// the tile ring (16-bit rows), or, where that is more, the patches through which the results leave
+constexpr int prefill_lds_bytes(bool sparse, int nw, int tt, int dh, int qh) {
+  const int ring = prefill_stages(sparse, nw) * 2 * 32 * tt * ROW_B, patches = nw * qh * 32 * (2 * dh + 8);
+  return ring > patches ? ring : patches;
+}
 template <bool SPARSE, int MODE, int NW, int TT, bool WIN, bool PACK, bool SPLIT, bool FP8, int DH, int QH>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(prefill_waves_per_simd(MODE, TT, DH), prefill_waves_per_simd(MODE, TT, DH))))
 void prefill_async_kernel(PrefillParams p) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   constexpr int BN = 32 * TT;                // keys per tile
@@ -244,7 +253,7 @@ void prefill_async_kernel(PrefillParams p) {
   // so all four are busy on four different resident tiles for exactly `local` steps and one new tile is requested per
   // step (four resident stages + one in flight).
   constexpr bool STAG = SPARSE && NW == 8;
-  constexpr int NST = STAG ? 5 : NW == 8 ? 4 : 2;   // LDS stages the copies land in
+  constexpr int NST = prefill_stages(SPARSE, NW);   // LDS stages the copies land in
   constexpr int UPW = FP8 ? 2 : 2 * UK / NW; // copy units per wave per tile (FP8: 8 raw rows of K, 8 of V)
   static_assert(!FP8 || (NW == 8 && MODE == 1 && !SPARSE && !PACK && TT == 2), "fp8 pools: 8-wave paged dense form only");
   constexpr int EB = FP8 ? 1 : 2;            // bytes per pool element
@@ -1185,7 +1194,7 @@ __global__ __launch_bounds__(256) void prefill_packed_reduce_kernel(PrefillParam
 
 template <bool SPARSE, int MODE, int NW, int TT = 2, bool WIN = false, bool PACK = false, bool SPLIT = false, bool FP8 = false, int DH = HD, int QH = 1>
 hipError_t launch_typed(const PrefillParams& p, hipStream_t s) {
-  constexpr int lds = (SPARSE && NW == 8 ? 5 : NW == 8 ? 4 : 2) * 2 * 32 * TT * ROW_B;
+  constexpr int lds = prefill_lds_bytes(SPARSE, NW, TT, DH, QH);
   constexpr int TOKW = DH == 64 ? 16 * NW : 32 * NW;      // query tokens per workgroup (plain form)
   static std::atomic<unsigned long long> configured{0};       // a bit per device: the attribute belongs to the device's own copy of the kernel
   int dev = 0;
@@ -1368,16 +1377,43 @@ static bool packed_takes_groups(const PrefillParams& p) {
   const long tokens = p.Hq == p.Hkv ? 1024 : 2048;      // on average per sequence
   return p.impl == 5 || p.window > 0 || p.total_q < tokens * p.B || (long)p.total_q * p.Hq < 256L * 2 * p.num_cus;
 }
+static int packed_groups(const PrefillParams& p) { return p.D == 64 ? (p.Hkv + 1) / 2 : p.Hkv; }
+// Workgroups per query tile and kv head (pair), with `heads` q heads per wave
+static int packed_heads_per_group(const PrefillParams& p, int heads) {
+  const int n_rep = p.Hq / p.Hkv, units = n_rep / heads;
+  return packed_takes_groups(p) ? 1 : p.D == 64 && p.Hkv == 1 ? (units + 1) / 2 : units;
+}
 static int packed_slots(const PrefillParams& p) {
   const bool groups = packed_takes_groups(p);
   const int mult = groups ? p.Hq / p.Hkv : 1;
   const int shift = p.D == 64 ? 6 : groups ? 7 : 8;
   return (int)(((long)mult * p.total_q) >> shift) + p.B;
 }
-static int packed_groups(const PrefillParams& p) { return p.D == 64 ? (p.Hkv + 1) / 2 : p.Hkv; }
-static int packed_heads_per_group(const PrefillParams& p) {      // workgroups per query tile and kv head (pair)
-  const int n_rep = p.Hq / p.Hkv, units = p.D == 64 ? n_rep / d64_heads_per_wave(p) : n_rep;
-  return packed_takes_groups(p) ? 1 : p.D == 64 && p.Hkv == 1 ? (units + 1) / 2 : units;
+// Key tiles (of 64 or 32 keys) and, at head dim 64, q heads per wave.
+// Head dim 64.  Two heads per wave read every tile for twice the matrix work.  With one, there are twice the workgroups, which calls of
+// fewer than four per CU want; and 32-key tiles (32 KB of LDS, 120 registers) let four be on a CU at once instead
+// of two, which covers each other's starts and ends where these weigh.  us, two heads / one head / one head and 32-key tiles (64 / 8
+// heads unless said; workgroups per CU with one head): 1 x 300 tokens (0.6) 15.7 / 13.0 / 13.2; 1 x 1 024 (2) 35.8 / 22.7 /
+// 26.4; 8 x 200-1 500, 16 / 1 heads (3.6) 50 / 31 / 36; 1 x 2 500, 16 / 4 heads (1.3) 78 / 44 / 54; 2 x 700 (2.9) 28.8 / 21.6 / 21.0; 4 x 500 (4.4)
+// 24.0 / 22.7 / 19.3; 1 x 2 000 (4.1) 65 / 54.6 / 51.3; 1 x 4 000 (8) 171 / 171 / 163; 32 x 17-256 (13) 33 / 38 / 27.8; 8 x 500-1 024 (12)
+// 64 / 70 / 57.5; 16 x 100-2 000 under a window of 128 (34) 117 / 148 / 110; 4 x 2 048 (16) 170 / - / 172; 8 x 500-4 000 under a window of 1 024
+// 435 / - / 440; 2 x 4 097-8 192 (24) 884 / 984 / 919.
+// Head dim 128, rows of a kv group.  The registers leave room for two workgroups per CU either way, and the gain is the
+// shorter first copy.  us, 64 / 32 keys: 32 x 17-256 tokens, 32 / 8 heads 28.7 / 27, 16 / 16 heads 22.8 / 21.8; 8 x 257-512 25.2 / 23.5; 8 x
+// 500-1 024 51.3 / 50.8, 24 x 16-2 048 110 / 111, 1 x 1 024 27.5 / 31.3, 8 x 64 behind 8 K 85 / 89.
+struct PackedForm { bool small; int heads; };      // 32-key tiles; q heads per wave
+static PackedForm packed_form(const PrefillParams& p) {
+  const int most = p.D == 64 ? d64_heads_per_wave(p) : 1;
+  if (p.splits > 1 || p.impl == 4 || p.impl == 6 || p.impl == 8) return {false, most};
+  long keys = std::max(p.total_q, p.total_k) / p.B;       // that a query may see: on average the whole sequence's, or the window's
+  if (p.window > 0) keys = std::min<long>(keys, p.window);
+  if (p.D == HD) return {packed_takes_groups(p) && p.window == 0 && (keys < 400 || p.impl == 7), 1};
+  if (p.impl == 7) return {true, 1};
+  const long tiles = (p.total_q >> 6) + (p.B + 1) / 2;     // about: the last tile of a sequence is half full
+  const long wgs = tiles * packed_groups(p) * packed_heads_per_group(p, 1);
+  if (wgs < 4L * p.num_cus) return {false, 1};
+  if (keys < 1024 || wgs < 8L * p.num_cus || most == 1) return {true, 1};
+  return {false, most};
 }
 
 int prefill_packed_splits(const PrefillParams& p, int num_cus) {
@@ -1393,7 +1429,7 @@ int prefill_packed_splits(const PrefillParams& p, int num_cus) {
   if (bound < 3 * mean) return 1;
   const int mult = p.D == HD ? p.Hq / p.Hkv : 1, shift = p.D == HD ? 7 : 6;
   const long tiles = std::max(1L, (((long)mult * p.total_q) >> shift) + p.B / 2);      // about: the last tile of a sequence is half full
-  const long wgs = tiles * packed_groups(p) * packed_heads_per_group(p), places = 2L * num_cus;
+  const long wgs = tiles * packed_groups(p) * packed_heads_per_group(p, p.D == 64 ? d64_heads_per_wave(p) : 1), places = 2L * num_cus;
   const long s = std::min((2 * places + wgs) / (2 * wgs), bound / (8 * 64));
   return s < 2 ? 1 : (int)std::min(s, 16L);
 }
@@ -1403,15 +1439,16 @@ hipError_t launch_prefill_packed(const PrefillParams& p0, hipStream_t s) {
   p.slots = packed_slots(p);
   p.n_rep = p.Hq / p.Hkv;
   p.kvg = packed_groups(p);
-  p.hpg = packed_heads_per_group(p);
+  const PackedForm form = packed_form(p);
+  p.hpg = packed_heads_per_group(p, form.heads);
   p.deal = p.kvg % 8 == 0 ? 0 : 8 % p.kvg == 0 ? 8 / p.kvg : -1;
   if ((long)p.slots * p.hpg > 0x7fffffffL) return hipErrorInvalidValue;
   p.by_rep.set(p.n_rep); p.by_hpg.set(p.hpg); p.by_kvg.set(p.kvg); p.by_head.set(p.slots * p.hpg); p.by_splits.set(p.splits);
   const bool split = p.splits > 1;
   if (split && (!p.ws_o || !p.ws_ml)) return hipErrorInvalidValue;
   if (p.D == 64) {       // (window 0 included: see launch_prefill_async)
-    const bool two = d64_heads_per_wave(p) == 2;
-    if (two) return split ? launch_typed<false, 2, 4, 2, true, false, true, false, 64, 2>(p, s)
+    if (form.small) return launch_typed<false, 2, 4, 1, true, false, false, false, 64>(p, s);
+    if (form.heads == 2) return split ? launch_typed<false, 2, 4, 2, true, false, true, false, 64, 2>(p, s)
                           : launch_typed<false, 2, 4, 2, true, false, false, false, 64, 2>(p, s);
     return split ? launch_typed<false, 2, 4, 2, true, false, true, false, 64>(p, s)
                  : launch_typed<false, 2, 4, 2, true, false, false, false, 64>(p, s);
@@ -1419,6 +1456,7 @@ hipError_t launch_prefill_packed(const PrefillParams& p0, hipStream_t s) {
   if (p.D != HD) return hipErrorInvalidValue;
   if (packed_takes_groups(p)) {
     if (p.window > 0) return split ? launch_typed<false, 2, 4, 2, true, true, true>(p, s) : launch_typed<false, 2, 4, 2, true, true>(p, s);
+    if (form.small) return launch_typed<false, 2, 4, 1, false, true>(p, s);
     return split ? launch_typed<false, 2, 4, 2, false, true, true>(p, s) : launch_typed<false, 2, 4, 2, false, true>(p, s);
   }
   // (the 8-wave form: dense long prompts that fill the device several times over; windows and splits are the other's)

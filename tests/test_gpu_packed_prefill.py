@@ -80,6 +80,27 @@ def test_ragged_prompts(pa, rng, debug_switch, Hq, Hkv, D, impl):
     _run(pa, rng, [1, 64, 0, 63, 129, 300, 2, 65, 33, 0], Hq, Hkv, D, tail=5)
 
 
+@pytest.mark.parametrize("form", [4, 6, 7])
+@pytest.mark.parametrize("Hq,Hkv,D", HEADS)
+def test_tile_forms(pa, rng, debug_switch, Hq, Hkv, D, form):
+    """64-key tiles, those with one q head per wave, 32-key tiles: whole prompts, prefixes, fewer keys than queries, a
+    window with sinks, whatever the sizes would choose."""
+    debug_switch(3, form)
+    debug_switch(6, 0)
+    _run(pa, rng, [1, 64, 0, 63, 129, 300, 2, 65, 33, 0], Hq, Hkv, D, tail=5)
+    _run(pa, rng, [40, 1, 130, 3, 70, 20], Hq, Hkv, D, kn=[400, 777, 130, 0, 5, 65], tail=3)
+    for window in (1, 40, 200):
+        _run(pa, rng, [150, 1, 300, 31], Hq, Hkv, D, kn=[150, 260, 700, 31], window=window, with_sinks=True)
+
+
+@pytest.mark.parametrize("n", [1, 20, 90])
+@pytest.mark.parametrize("Hq,Hkv,D", [(16, 8, 64), (6, 2, 64), (16, 4, 128)])
+def test_forms_the_sizes_choose(pa, rng, Hq, Hkv, D, n):
+    """Calls of a few and of many workgroups, short and long."""
+    _run(pa, rng, [int(x) for x in rng.integers(100, 300, n)], Hq, Hkv, D)
+    _run(pa, rng, [int(x) for x in rng.integers(1, 60, 2 * n)] + [1500], Hq, Hkv, D)
+
+
 @pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (64, 8, 64), (16, 2, 128), (16, 16, 64)])
 def test_strided_rows(pa, rng, Hq, Hkv, D):
     _run(pa, rng, [100, 1, 200, 17], Hq, Hkv, D, strided=True)
