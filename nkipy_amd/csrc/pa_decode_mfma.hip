@@ -486,13 +486,15 @@ struct DecodeWave {
   // Pool rows of tokens t0 and t0+16 (the two 16-token halves of a tile each lie
   // inside one block: block_size is a power of two >= 16, t0 a multiple of 32).
   struct TileRows { long row0, row1; int blk0, blk1, lmax; };
-  __device__ __forceinline__ TileRows tile_rows(int t0) const {
+  // the table's entries for the two halves of the tile at t0 (any t0: past the context they are the last block's)
+  struct TileBlocks { int b0, b1; };
+  __device__ __forceinline__ TileBlocks tile_blocks(int t0) const {
+    return {table[min(t0, last) >> p.block_shift], table[min(t0 + 16, last) >> p.block_shift]};        // wave-uniform
+  }
+  __device__ __forceinline__ TileRows tile_rows(int t0, const TileBlocks& e) const {
     TileRows tr;
-    const int t1 = min(t0 + 16, last);             // wave-uniform
-    const int blk0 = table[t0 >> p.block_shift];
-    const int blk1 = table[t1 >> p.block_shift];
-    tr.blk0 = min(max(blk0, 0), p.num_blocks - 1);
-    tr.blk1 = min(max(blk1, 0), p.num_blocks - 1);
+    tr.blk0 = min(max(e.b0, 0), p.num_blocks - 1);
+    tr.blk1 = min(max(e.b1, 0), p.num_blocks - 1);
     const int bmask = p.block_size - 1;
     tr.row0 = (long)tr.blk0 * p.block_size + (t0 & bmask);
     tr.row1 = (long)tr.blk1 * p.block_size + ((t0 + 16) & bmask);
@@ -528,8 +530,9 @@ struct DecodeWave {
   // Loads of the tile starting at token t0.  Rows past the context are
   // redirected to the last valid token so that no stale pool bytes (which could
   // be NaN patterns) ever reach the matrix cores.
-  __device__ __forceinline__ void load_k(KT& tl, int t0) const {
-    const TileRows tr = tile_rows(t0);
+  __device__ __forceinline__ void load_k(KT& tl, int t0) const { load_k(tl, t0, tile_blocks(t0)); }
+  __device__ __forceinline__ void load_k(KT& tl, int t0, const TileBlocks& e) const {
+    const TileRows tr = tile_rows(t0, e);
     if (FP8) {
       tl.ksc[0] = p.k_scale[(long)tr.blk0 * p.Hkv + hk];
       tl.ksc[1] = p.k_scale[(long)tr.blk1 * p.Hkv + hk];
@@ -584,8 +587,9 @@ struct DecodeWave {
       out[d] = k_first_half ? a : b;
     }
   }
-  __device__ __forceinline__ void load_v(VT& tl, int t0) const {
-    const TileRows tr = tile_rows(t0);
+  __device__ __forceinline__ void load_v(VT& tl, int t0) const { load_v(tl, t0, tile_blocks(t0)); }
+  __device__ __forceinline__ void load_v(VT& tl, int t0, const TileBlocks& e) const {
+    const TileRows tr = tile_rows(t0, e);
     if (FP8) {
       tl.vsc[0] = p.v_scale[(long)tr.blk0 * p.Hkv + hk];
       tl.vsc[1] = p.v_scale[(long)tr.blk1 * p.Hkv + hk];
@@ -869,27 +873,40 @@ struct DecodeWave {
       return;
     }
     VT vb;
+    // int8: the table's entries are fetched a tile ahead of the loads that need them (us, 64 / 8 heads of 64: 8 sequences of
+    // 500-2 048 tokens, T = 4, 17.8 -> 16.7, 64 sequences of 512-8 192 75.8 -> 70.6, 32 of 512-4 096, T = 8, 64.9 -> 61.8; bf16 pools,
+    // 64 of 512-8 192, 32 / 8 heads of 128, 166.9 -> 170.5).  A third tile in flight brought nothing.
+    TileBlocks e = tile_blocks(t + (I8 ? t_step : 0));
+    auto take = [&](int at) __attribute__((always_inline)) {        // the entries of the tile at `at`, which is loaded now
+      if (!I8) return tile_blocks(at);
+      const TileBlocks now = e;
+      e = tile_blocks(at + t_step);
+      return now;
+    };
     while (i + 2 < n) {
       if (lockstep) __builtin_amdgcn_s_barrier();
-      load_k(kb, t + t_step);
+      const TileBlocks eb = take(t + t_step);
+      load_k(kb, t + t_step, eb);
       patch_new_rows(ka, va, t);
       scores_softmax(ka, va, t, t_end);
-      load_v(vb, t + t_step);
+      load_v(vb, t + t_step, eb);
       accumulate_pv(va);
       if (lockstep) __builtin_amdgcn_s_barrier();
-      load_k(ka, t + 2 * t_step);
+      const TileBlocks ea = take(t + 2 * t_step);
+      load_k(ka, t + 2 * t_step, ea);
       patch_new_rows(kb, vb, t + t_step);
       scores_softmax(kb, vb, t + t_step, t_end);
-      load_v(va, t + 2 * t_step);
+      load_v(va, t + 2 * t_step, ea);
       accumulate_pv(vb);
       i += 2;
       t += 2 * t_step;
     }
     if (i + 1 < n) {
-      load_k(kb, t + t_step);
+      const TileBlocks eb = take(t + t_step);
+      load_k(kb, t + t_step, eb);
       patch_new_rows(ka, va, t);
       scores_softmax(ka, va, t, t_end);
-      load_v(vb, t + t_step);
+      load_v(vb, t + t_step, eb);
       accumulate_pv(va);
       patch_new_rows(kb, vb, t + t_step);
       scores_softmax(kb, vb, t + t_step, t_end);
