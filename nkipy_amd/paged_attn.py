@@ -107,10 +107,15 @@ class _NoGuard:
 _NO_GUARD = _NoGuard()
 
 
+# (the public calls first make sure that torch's device runtime is up, which a device tensor in hand says already)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_is_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
+
+
 def _on(device):
     """Context in which `device` is the current one for a launch; nothing to switch when it already is
     (the usual case, and the switch costs a few microseconds of a call that launches ten-microsecond kernels)."""
-    return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _NO_GUARD if _current_device() == device.index else torch.cuda.device(device)
 
 
 def _ptr(t):
@@ -132,12 +137,15 @@ def _kv_code(cache, scale_given):
     return _DTYPE_CODE[cache.dtype]
 
 
-def _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, what="KV"):
-    """The scale tables of a pool of codes: one float per (block, kv head) for fp8, per (token, kv head) for int8."""
+def _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, what="KV", on_device=False):
+    """The scale tables of a pool of codes: one float per (block, kv head) for fp8, per (token, kv head) for int8.
+    on_device: the caller has been through `_all_on` with them."""
     shape, text = ((num_blocks, Hkv), "[num_blocks, Hkv]") if kv_code == FP8 else \
                   ((num_blocks, Hkv, block_size), "[num_blocks, Hkv, block_size]")
     if not (k_scale is not None and v_scale is not None):
         raise ValueError(f"{'fp8' if kv_code == FP8 else 'int8'} {what} needs both k_scale and v_scale")
+    if on_device and k_scale.shape == shape == v_scale.shape and k_scale.dtype == v_scale.dtype == torch.float32:
+        return
     for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
         _need_device(n, t)
         if t.dtype != torch.float32 or t.shape != shape:
@@ -148,9 +156,10 @@ def _check_paging(k_cache, v_cache, block_tables, seq_lens, B):
     _check(k_cache.dim() == 4, "k_cache must be [num_blocks, block_size, Hkv, D]")
     _check(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype,
            "v_cache must match k_cache in shape and dtype")
-    _check(block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.dtype == torch.int32,
+    table = block_tables.shape
+    _check(len(table) == 2 and table[0] == B and block_tables.dtype == torch.int32,
            "block_tables must be int32 [B, max_blocks_per_seq]")
-    _check(block_tables.shape[1] > 0, "block_tables needs at least one column")
+    _check(table[1] > 0, "block_tables needs at least one column")
     _check(seq_lens.shape == (B,) and seq_lens.dtype == torch.int32, "seq_lens must be int32 [B]")
 
 
@@ -206,7 +215,7 @@ def _workspace(device, nbytes, stream=None):
     graphs concurrently pass a `workspace=` of their own per graph, sized with the *_workspace_bytes functions,
     and keep it alive."""
     key = (device, (stream or _stream_ptr(device)).value)
-    if (device.type if isinstance(device, torch.device) else torch.device(device).type) == "cuda" and torch.cuda.is_current_stream_capturing():
+    if (device.type if isinstance(device, torch.device) else torch.device(device).type) == "cuda" and _is_capturing():
         buf = _graph_workspaces.get(key)
         if buf is None or buf.numel() < nbytes:
             if buf is not None:
@@ -313,7 +322,7 @@ def decode(q, k_cache, v_cache, block_tables, seq_lens, scale, *, k_scale=None, 
     if kv_code in (FP8, I8):
         if q_code != BF16:
             raise ValueError(f"{'fp8' if kv_code == FP8 else 'int8'} KV needs bfloat16 q")
-        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv)
+        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, on_device=True)
         if not (kv_code == FP8 or verify_supported(1, D, block_size)):
             raise ValueError(f"int8 KV needs head_dim 64 or 128 and a power-of-two block size >= 16 (D={D}, block_size={block_size})")
     else:
@@ -443,7 +452,7 @@ def prefill(q, k_cache, v_cache, block_tables, seq_lens, query_lens, scale, *, k
     if Hq % Hkv != 0:
         raise ValueError(f"Hq={Hq} is not a multiple of Hkv={Hkv}")
     if kv_code in (FP8, I8):
-        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv)
+        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, on_device=True)
     else:
         _check(not scaled, "k_scale/v_scale are only valid with an fp8 or int8 KV cache")
     _check(route in (None, "verify", "tiled"), "route must be None, 'verify' or 'tiled'")
@@ -746,7 +755,7 @@ def kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens,
     _check(seq_lens.shape == (B,) and seq_lens.dtype == torch.int32, "seq_lens must be int32 [B]")
     _check(query_lens.shape == (B,) and query_lens.dtype == torch.int32, "query_lens must be int32 [B]")
     if kv_dtype in (FP8, I8):
-        _check_scales(kv_dtype, k_scale, v_scale, num_blocks, block_size, Hkv, "pool")
+        _check_scales(kv_dtype, k_scale, v_scale, num_blocks, block_size, Hkv, "pool", True)
     else:
         _check(k_scale is None and v_scale is None, "k_scale / v_scale are for float8 and int8 pools only")
     if not (kv_dtype != I8 and not packed or D in (32, 64, 128, 256)):
@@ -794,7 +803,7 @@ def read_kv(k_cache, v_cache, block_tables, seq_lens, cu_seqlens, total_tokens=N
     kv_code = _kv_code(k_cache, scaled)
     _check(kv_code != F32, "read_kv takes bfloat16, float8_e4m3fn / uint8 and int8 pools")
     if kv_code in (FP8, I8):
-        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, "pool")
+        _check_scales(kv_code, k_scale, v_scale, num_blocks, block_size, Hkv, "pool", True)
     else:
         _check(not scaled, "k_scale / v_scale are for float8 and int8 pools only")
     if D % 8 != 0:
