@@ -290,6 +290,7 @@ struct DecodeParams {
   int partition_size, num_partitions, max_seq_len;
   float scale_log2e;
   int head_major;           // fixed-partition grid order: kv head fastest (1) or partition fastest (0)
+  int line_group;           // ... and how many neighbouring head slots share an XCD (set by the launcher)
   int bal_hsw, bal_ns, bal_gv;  // balanced schedule: head slots and chunks per workgroup, total chunks
   int bal_lockstep;         // keep the head waves of a workgroup on the same tile with a barrier
   QTransform qt;            // balanced schedule only: Q rows are normed and rotated as they are loaded

@@ -41,6 +41,7 @@
 //
 // Math restated: attention.py:112-144 + softmax.py:4-6 in one pass; the merge
 // of partitions is  m = max m_i, l = sum l_i 2^(m_i-m), o = sum o_i l_i 2^(m_i-m)/l.
+#include <algorithm>
 #include <type_traits>
 
 #include "pa_common.h"
@@ -405,7 +406,7 @@ struct DecodeWave {
   // int8: the row's values become 16-bit integers under a scale of their own, absmax / 32 512, in two limbs of 8 bits (256
   // high + low, both signed): the score product is then the integer matrix instruction's on the codes as they lie in
   // memory, exact, where a conversion to bf16 costs three vector instructions for two codes (64 / 8 heads of 128, 64
-  // sequences of 1 024-32 768 tokens: 203 -> 194 us, 6.0 TB/s; 64 / 8 heads of 64, 64 of 512-8 192: 80 -> 75.5).  An element is rounded at
+  // sequences of 1 024-32 768 tokens: 203 -> 194 us, 6.0 TB/s; 64 / 8 heads of 64, 64 of 512-8 192: 80 -> 75.5, now 70.6).  An element is rounded at
   // most half a step, 2^-16 of the row's largest (2^-121 where that is less: steps below 2^-120 have no reciprocal); a bf16 value at least 2^-8 of the largest is not rounded at all.  Slot
   // limb * KLD + s holds limb 0 (high) or 1 (low) of the 16 elements that lane (g, .) has of step s.  A row with an
   // infinity or a NaN gets the scale NaN.
@@ -1033,8 +1034,15 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 1 : 2) void decode_mfma_kernel(De
   constexpr int VEC = W::VEC;
   constexpr int OSTRIDE = D + 16;   // LDS row stride (floats) for the merge
 
-  const int part = p.head_major ? blockIdx.y : blockIdx.x, b = blockIdx.z;
-  const int hidx = p.head_major ? blockIdx.x : blockIdx.y;
+  int part = p.head_major ? blockIdx.y : blockIdx.x, b = blockIdx.z;
+  int hidx = p.head_major ? blockIdx.x : blockIdx.y;
+  if (p.line_group > 1) {      // (see line_group_of; consecutive workgroups go to consecutive XCDs)
+    const int id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z), k = id >> 3, turn = k / p.line_group;
+    const int unit = 8 * turn + (id & 7), groups = gridDim.x / p.line_group, rest = unit / groups;
+    hidx = (unit - rest * groups) * p.line_group + k - turn * p.line_group;
+    b = rest / gridDim.y;
+    part = rest - b * gridDim.y;
+  }
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1493,10 +1501,25 @@ __global__ __launch_bounds__(256) void decode_balanced_reduce_kernel(DecodeParam
   }
 }
 
+// Head slots that read the same 128-byte lines of the pool: the 16-row groups of a kv head, and the heads whose rows share a
+// line (64 codes: two).  Dealt out one by one they sit on different XCDs, each of which fetches the line for its own L2
+// (8 sequences of 500-2 048 tokens, T = 4, 64 / 8 heads of 64, int8: 39 MB fetched of a pool of 10); so they are given to one
+// XCD, next to each other, where the units of such slots fill the eight XCDs evenly.  us per call, one by one / together: 32 / 8 heads of
+// 128, 16 sequences of 500-1 024, T = 8, int8 17.4 / 16.9, bf16 22.0 / 17.8; 1 of 4 096, T = 8, int8 15.9 / 15.1, fp8 14.8 / 13.9;
+// 64 / 8 heads of 64, 16 of 500-1 024, T = 4, int8 14.8 / 13.7, bf16 13.8 / 12.1.  Calls of fewer than 128 workgroups are left alone
+// (64 of them: 1 of 1 024, T = 4, 8.8 / 9.1; 1 of 4 096, T = 1, 10.8 / 11.0).
+static int line_group_of(const DecodeParams& p, int slots, int row_bytes) {
+  const int heads = std::max(1, 128 / row_bytes), g = slots / p.Hkv * heads;
+  const long workgroups = (long)slots * p.num_partitions * p.B;
+  if (!p.head_major || g <= 1 || p.Hkv % heads || workgroups < 128 || workgroups > 0x7fffffffL) return 1;
+  return workgroups / g % 8 == 0 ? g : 1;
+}
 template <int D, int KV>
-hipError_t launch_typed(const DecodeParams& p, int waves, hipStream_t s) {
+hipError_t launch_typed(const DecodeParams& p0, int waves, hipStream_t s) {
+  DecodeParams p = p0;
   const int n_rep = p.Hq / p.Hkv;
   const int slots = head_slots_of(p);                  // Hkv x 16-row groups of a kv head's rows
+  p.line_group = line_group_of(p, slots, KV == KV_BF16 ? 2 * D : D);
   dim3 grid(p.num_partitions, slots, p.B);
   if (p.head_major) grid = dim3(slots, p.num_partitions, p.B);
   if (p.query_lens) {      // multi-token rows: the four-wave form
