@@ -6,7 +6,8 @@
 //   bf16   the bits as they are
 // each product in float32, rounded once.
 //
-// Pure streaming, HBM bound: a byte in, two bytes out (four with bf16).  A workgroup takes 16 tokens of one sequence; a
+// Pure streaming, HBM bound: a byte in, two bytes out (four with bf16).  270 K tokens of 8 heads of 128, int8: 316-329 us,
+// 5.1-5.3 TB/s (a copy of 2 GiB reaches 4.9); 2 K tokens 5.5 us.  A workgroup takes 16 tokens of one sequence; a
 // token's heads are adjacent in the pool and in the output, so consecutive lanes walk whole rows.  The sequence of a
 // workgroup is found by bisection (packed_find); rows of the output that no token falls on are left as they are.
 #include "pa_common.h"

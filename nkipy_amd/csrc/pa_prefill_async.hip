@@ -1365,7 +1365,7 @@ hipError_t launch_prefill_async(const PrefillParams& p, int waves, hipStream_t s
 }
 
 // ---- packed form ---------------------------------------------------------------------------------------------
-// Workgroup shapes.  Head dim 64: 4 waves, 64 tokens of two kv heads (against 8 waves and 128 tokens, us: 16 windowed
+// Workgroup shapes (times with 64-key tiles, and two q heads per wave at head dim 64; packed_form below chooses between these).  Head dim 64: 4 waves, 64 tokens of two kv heads (against 8 waves and 128 tokens, us: 16 windowed
 // prompts of 100-2 000 tokens 134 / 171, 32 prompts of 17-256 37 / 46, 2 of 4 097-8 192 891 / 965).  Head dim 128: 4 waves
 // with 128 rows of a kv group (its q heads' rows share the tile), two workgroups per CU, or 8 waves with 256 tokens of
 // one q head, one per CU: half the copies per product, for long prompts that fill the device twice over.  us, 4 / 8 waves,
