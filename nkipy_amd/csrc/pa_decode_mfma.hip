@@ -163,6 +163,12 @@ struct DecodeWave {
   const char* kbase;
   const char* vbase;
   long row_stride;           // bytes between consecutive tokens of a block
+  // int8: where this lane's pieces lie in the 16 K rows (V: in the first of four V rows) of half a tile.  Rows past the context
+  // are loaded as they lie: a code is finite whatever it is, and what it meets is masked by selection.  So the addresses
+  // are wave-uniform but for these, where clamping each row to the context took a third of a tile's vector instructions (us: 8
+  // sequences of 500-2 048, T = 4, 64 / 8 heads of 64, 16.6 -> 15.1; 32 of 1 000-4 096, T = 16, 32 / 8 heads of 128, 88 -> 81.7; 64 of
+  // 1 024-32 768, 64 / 8 heads of 128, 196.6 -> 194.7).
+  uint32_t k_off, v_off;
   int last;                  // ctx - 1 of the current sequence
   int jbase;                 // first row of this wave inside its kv group
   // SK: K travels as whole 128-byte lines (see load_k); where this lane's chunk of steps with even / odd s sits
@@ -206,6 +212,10 @@ struct DecodeWave {
     kperm_addr[0] = 4 * (8 * (krow & 7) + g);
     kperm_addr[1] = 4 * (8 * (krow & 7) + 4 + g);
     row_stride = (long)p.Hkv * D * ESZ;
+    if constexpr (I8) {
+      k_off = (uint32_t)(krow * row_stride + g * 16);
+      v_off = (uint32_t)(4 * g * row_stride + r * (VEC * ESZ));
+    }
     kbase = (const char*)p.k_cache + (long)hk * D * ESZ;
     vbase = (const char*)p.v_cache + (long)hk * D * ESZ;
     new_t0 = -1;
@@ -556,6 +566,16 @@ struct DecodeWave {
         }
       return;
     }
+    if constexpr (I8) {
+      // (see k_off)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const char* half = kbase + (u ? tr.row1 : tr.row0) * row_stride;
+#pragma unroll
+        for (int s = 0; s < KLD; ++s) VecLoad<4, kStreamK>::get(half + k_off + 64 * s, tl.k[u][s]);
+      }
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int tl_ = min(16 * u + krow, tr.lmax);
@@ -594,6 +614,14 @@ struct DecodeWave {
     if (FP8) {
       tl.vsc[0] = p.v_scale[(long)tr.blk0 * p.Hkv + hk];
       tl.vsc[1] = p.v_scale[(long)tr.blk1 * p.Hkv + hk];
+    }
+    if constexpr (I8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const char* row = vbase + ((j < 4 ? tr.row0 : tr.row1) + (j & 3)) * row_stride;
+        VecLoad<VW, SV>::get(row + v_off, tl.v[j]);
+      }
+      return;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
