@@ -322,6 +322,30 @@ def test_verify_rows_per_wave(pa, rng, debug_switch, rows):
         debug_switch(5, 0)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,T,B", [(64, 8, 64, 4, 8), (64, 8, 64, 1, 16), (32, 8, 128, 8, 16), (32, 2, 128, 16, 16), (40, 4, 64, 3, 24), (9, 3, 64, 8, 32), (16, 1, 128, 8, 16)])
+def test_slots_that_share_lines(pa, rng, debug_switch, Hq, Hkv, D, T, B):
+    """Where the head slots that read the same lines go to one XCD (calls of at least 128 workgroups), the results are those
+    of the other grid order bit for bit, for every pool type."""
+    ctxs = [1024] + [int(c) for c in rng.integers(T, 1024, B - 1)]
+    pool = int8_pool(rng, ctxs, 32, Hkv, D)
+    q = bf16(rng.standard_normal((B, T, Hq, D)))
+    tables, lens, qlens = dev(pool["tables"]), dev(np.asarray(ctxs, np.int32)), dev(np.asarray([T - (i % 2) * (T > 1) for i in range(B)], np.int32))
+    codes = [dev(pool[n]) for n in "kv"]
+    pools = [(codes, {"k_scale": dev(pool["ks"]), "v_scale": dev(pool["vs"])}), ([c.to(torch.bfloat16) for c in codes], {}),
+             ([c.view(torch.uint8).bitwise_and(0x77).view(torch.float8_e4m3fn) for c in codes],
+              {n: torch.full((pool["blocks"], Hkv), 0.02, device="cuda") for n in ("k_scale", "v_scale")})]
+    for kv, scales in pools:
+        got = []
+        for order in (1, 0):
+            debug_switch(2, order)
+            try:
+                got.append(pa.decode(q[:, 0].contiguous(), *kv, tables, lens, 0.05, max_seq_len=1024, **scales) if T == 1 else
+                           pa.verify(q, *kv, tables, lens, qlens, 0.05, max_seq_len=1024, **scales))
+            finally:
+                debug_switch(2, 1)
+        assert torch.isfinite(got[0]).all() and torch.equal(*got)
+
+
 def test_a_masked_token_of_any_scale_leaves_no_trace(pa, rng):
     """Tokens that a window hides may have NaN scales (a row that held an infinity): they must not reach the result."""
     D, bs, Hkv, Hq, c = 128, 16, 2, 8, 300
