@@ -141,20 +141,25 @@ class PagedKVCache:
         n_tab = max_seqs * max_blocks_per_seq
         self._off_lens = (n_tab + 63) // 64 * 64
         self._off_qlens = self._off_lens + (max_seqs + 63) // 64 * 64
-        # int8 caches: where each slot's context begins among the rows of all slots that take part in the step, for the
-        # chunks that read the cache back (PagedAttention.attend)
+        # int8 caches: where each slot's context begins among the rows of all slots that take part in the step, and where
+        # its rows begin among the step's [max_seqs, tokens] ones, for the chunks that read the cache back
+        # (PagedAttention.attend).  Both are published with the step: a chunk that is captured into a graph before any
+        # other call of its length finds them in place, as does an eager call behind that capture
         self._off_starts = self._off_qlens + ((max_seqs + 63) // 64 * 64 if self.int8 else max_seqs)
-        self._host_meta = np.zeros(self._off_starts + (max_seqs + 1 if self.int8 else 0), dtype=np.int32)
+        self._off_qstarts = self._off_starts + (max_seqs + 64) // 64 * 64
+        self._host_meta = np.zeros(self._off_qstarts + max_seqs + 1 if self.int8 else self._off_starts, dtype=np.int32)
         self._host_tables = self._host_meta[:n_tab].reshape(max_seqs, max_blocks_per_seq)
         self._host_tables[:] = -1
         self._host_lens = self._host_meta[self._off_lens:self._off_lens + max_seqs]
         self._host_qlens = self._host_meta[self._off_qlens:self._off_qlens + max_seqs]
-        self._host_starts = self._host_meta[self._off_starts:]
+        self._host_starts = self._host_meta[self._off_starts:self._off_starts + max_seqs + 1]
+        self._host_qstarts = self._host_meta[self._off_qstarts:]
         self._meta = torch.from_numpy(self._host_meta).to(self.device)
         self.block_tables = self._meta[:n_tab].view(max_seqs, max_blocks_per_seq)
         self.seq_lens = self._meta[self._off_lens:self._off_lens + max_seqs]
         self.query_lens = self._meta[self._off_qlens:self._off_qlens + max_seqs]
-        self.row_starts = self._meta[self._off_starts:] if self.int8 else None
+        self.row_starts = self._meta[self._off_starts:self._off_starts + max_seqs + 1] if self.int8 else None
+        self.query_starts = self._meta[self._off_qstarts:] if self.int8 else None
         self._stage = self._stage_done = None
         self._stage_at = 0
         if self.device.type == "cuda":
@@ -228,12 +233,14 @@ class PagedKVCache:
         if any(n < 0 or n > tokens for n in query_lens):
             raise ValueError("query_lens must lie in [0, tokens]")
         active = [s for s in range(self.max_seqs) if query_lens[s] > 0]
-        before = self._host_qlens.copy()
+        before = self._host_qlens.copy(), self._host_qstarts.copy()
         self._host_qlens[:] = query_lens
+        if self.int8:
+            self._host_qstarts[:] = np.arange(self.max_seqs + 1) * tokens
         try:
             self.extend(active, [query_lens[s] for s in active])      # publishes the query lengths with the rest
         except Exception:
-            self._host_qlens[:] = before
+            self._host_qlens[:], self._host_qstarts[:] = before
             raise
         self.step_tokens = tokens
 
@@ -326,8 +333,7 @@ class PagedAttention:
             raise ValueError(f"o_weight must be [{n_heads * cache.head_dim}, hidden], got {tuple(o_weight.shape)}")
         self._out: Dict[int, torch.Tensor] = {}
         self._proj: Dict[int, torch.Tensor] = {}
-        self._q: Dict[int, torch.Tensor] = {}            # chunks over an int8 cache: transformed queries, first rows
-        self._starts: Dict[int, torch.Tensor] = {}
+        self._q: Dict[int, torch.Tensor] = {}            # chunks over an int8 cache: transformed queries
         # decode / verify steps prepared once per (T, length bound, storage of xq / xk / xv): a loop that feeds the
         # layer from the same buffers every step pays the argument checks once (see paged_attn.PreparedStep)
         self._steps: Dict[tuple, tuple] = {}
@@ -485,14 +491,11 @@ class PagedAttention:
         else:
             paged_attn.kv_write(xk, xv, kc, vc, c.block_tables, c.seq_lens, c.query_lens, k_scale=ks, v_scale=vs)
             q = xq
-        starts = self._starts.get(T)
-        if starts is None:
-            starts = self._starts[T] = torch.arange(0, (B + 1) * T, T, dtype=torch.int32, device=c.device)
         # rows for the contexts: what the host knows of this step, or, captured into a graph that will be replayed on
         # other lengths, what the bound admits
         rows = B * bound if capturing else int(c._host_starts[-1])
         k, v = paged_attn.read_kv(kc, vc, c.block_tables, c.seq_lens, c.row_starts, rows, k_scale=ks, v_scale=vs)
-        paged_attn.packed_prefill(q.reshape(B * T, self.n_heads, c.head_dim), k, v, starts, self.scale, cu_seqlens_k=c.row_starts,
+        paged_attn.packed_prefill(q.reshape(B * T, self.n_heads, c.head_dim), k, v, c.query_starts, self.scale, cu_seqlens_k=c.row_starts,
                                   query_lens=c.query_lens, seq_lens=c.seq_lens, max_seq_len=bound, sinks=self.sinks,
                                   sliding_window=self.sliding_window, out=out.view(B * T, self.n_heads, c.head_dim))
         if self.o_weight is None:
