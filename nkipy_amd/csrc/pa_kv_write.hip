@@ -495,9 +495,9 @@ __global__ __launch_bounds__(WG) void kv_write_rows_kernel(KvWriteParams p) {
   }
   const int t = (tile << p.tok_shift) + tok;
   const int seq = min(p.seq_lens[b], p.max_blocks * p.block_size);
-  const int start = seq - tq;
-  const int pos = start + t;
-  bool live = h < p.Hkv && t >= 0 && t < tq && start >= 0;
+  // (compared, not subtracted: the difference of a length near the smallest integer wraps round to a position far behind the table)
+  bool live = h < p.Hkv && t >= 0 && t < tq && seq >= tq;
+  const int pos = live ? seq - tq + t : 0;
   int blk = -1, in_blk = 0;
   if (live) {
     const int jb = pos / p.block_size;
