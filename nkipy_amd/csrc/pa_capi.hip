@@ -978,6 +978,10 @@ int pa_packed_prefill(const void* q, const void* k, const void* v, long q_stride
   if (k_stride > 0x0fffffffL || v_stride > 0x0fffffffL) return fail_arg("%s: a token stride exceeds 2^28 elements", who);
   if ((long)total_q * (Hq / Hkv) + num_seqs > 0x7fff0000L)
     return fail_arg("%s: %d rows of %d q heads per kv head exceed 2^31", who, total_q, Hq / Hkv);
+  if ((long)total_q + total_k > 0x7fffffffL) return fail_arg("%s: %d query and %d key rows exceed 2^31 together", who, total_q, total_k);
+  // A window of all keys there are is none.  (Kept, its length behind a query that lies before its sequence's first key --
+  // fewer keys than queries -- would be a position past the smallest integer; the two row counts bound what is left.)
+  if (sliding_window >= total_k) sliding_window = 0;
   if (num_seqs == 0 || total_q == 0) return 0;
   if (!q || !cu_seqlens_q || !out || (total_k > 0 && (!k || !v)) || !cu_seqlens_k) return fail_arg("%s: null pointer argument", who);
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return fail_arg("%s: q, k, v and out must be 16-byte aligned", who);

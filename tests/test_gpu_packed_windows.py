@@ -1,0 +1,31 @@
+"""Packed prompts under windows at the ends of their range, and in front of prefixes."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_attention_oracle as O
+from tests.int8_kv_lib import bf16, dev
+from tests.test_gpu_packed_prefill import _run, _starts, debug_switch, pa  # noqa: F401  (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 140])
+@pytest.mark.parametrize("split", [0, 1, 3])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (8, 4, 64), (3, 1, 64)])
+def test_the_longest_windows(pa, rng, debug_switch, Hq, Hkv, D, split, window):  # noqa: F811
+    """A window longer than any context is none, for sequences with fewer keys than queries too: the reach of their first
+    queries lies before the first key, and a window's length behind it is past the smallest integer."""
+    debug_switch(6, split)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    _run(pa, rng, [40, 1, 130, 300, 70, 20], Hq, Hkv, D, kn=[400, 777, 127, 3, 5, 65], tail=3, window=window, workspace=ws)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (8, 2, 64)])
+def test_a_window_of_all_rows_is_none(pa, rng, Hq, Hkv, D):  # noqa: F811
+    n = [90, 33, 200]
+    q, k, v = (bf16(O.round_to_bf16(rng.standard_normal((sum(n), h, D)).astype(np.float32))) for h in (Hq, Hkv, Hkv))
+    cu = dev(_starts(n))
+    want = pa.packed_prefill(q, k, v, cu, 0.1)
+    for window in (sum(n), sum(n) + 1, 2 ** 31 - 1):
+        assert torch.equal(pa.packed_prefill(q, k, v, cu, 0.1, sliding_window=window), want)
