@@ -245,9 +245,12 @@ int pa_prefill(const void* q, const void* k_cache, const void* v_cache,
  *   max_seq_len   0, or a host-known upper bound of a sequence's keys (a hint: see the workspace)
  *   workspace     NULL, or pa_packed_prefill_workspace_bytes(...) bytes (16-byte aligned; 0 = none needed): with it, a
  *                 call of few queries over many keys splits the keys of a query tile over several workgroups and merges
- *                 their results in a second kernel
+ *                 their results in a second kernel.  ..._for answers for a call under a sliding window, which has fewer
+ *                 keys to split
  */
 size_t pa_packed_prefill_workspace_bytes(int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len);
+size_t pa_packed_prefill_workspace_bytes_for(int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len,
+                                             int sliding_window);
 int pa_packed_prefill(const void* q, const void* k, const void* v, long q_stride, long k_stride, long v_stride,
                       const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* query_lens,
                       const int32_t* seq_lens, void* out, void* workspace, size_t workspace_bytes,

@@ -137,7 +137,7 @@ using namespace pa;
 
 extern "C" {
 
-int pa_version(void) { return 400; }   // 0.4.0: int8 pools, pa_kv_write_packed, pa_read_kv, pa_packed_prefill
+int pa_version(void) { return 500; }   // 0.5.0: pa_packed_prefill_workspace_bytes_for (0.4.0: int8 pools, packed writes and prompts, pa_read_kv)
 
 const char* pa_last_error(void) { return tl_error; }
 
@@ -938,23 +938,32 @@ int pa_prefill(const void* q, const void* k_cache, const void* v_cache,
   return check_hip(e, "pa_prefill launch");
 }
 
-static void fill_packed_shape(PrefillParams& p, int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len) {
+static void fill_packed_shape(PrefillParams& p, int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len,
+                              int sliding_window) {
   memset(&p, 0, sizeof(p));
   p.B = num_seqs; p.total_q = total_q; p.total_k = total_k; p.Hq = Hq; p.Hkv = Hkv; p.D = D;
   p.block_shift = -1;
   p.len_bound = max_seq_len;
+  // A window of all keys there are is none.  (Kept, its length behind a query that lies before its sequence's first key --
+  // fewer keys than queries -- would be a position past the smallest integer; the two row counts bound what is left.)
+  p.window = sliding_window >= total_k ? 0 : sliding_window;
   p.impl = g_prefill_impl.load();
   p.num_cus = current_num_cus();
 }
 
-size_t pa_packed_prefill_workspace_bytes(int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len) {
+size_t pa_packed_prefill_workspace_bytes_for(int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len,
+                                             int sliding_window) {
   if (num_seqs <= 0 || total_q <= 0 || total_k <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (D != 64 && D != 128) ||
-      (long)total_q * (Hq / Hkv) + num_seqs > 0x7fff0000L)
+      sliding_window < 0 || (long)total_q * (Hq / Hkv) + num_seqs > 0x7fff0000L)
     return 0;
   PrefillParams p;
-  fill_packed_shape(p, num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len);
+  fill_packed_shape(p, num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len, sliding_window);
   const int want = prefill_packed_splits(p, p.num_cus);
   return want > 1 ? (size_t)total_q * Hq * want * ((size_t)D + 2) * sizeof(float) : 0;
+}
+
+size_t pa_packed_prefill_workspace_bytes(int num_seqs, int total_q, int total_k, int Hq, int Hkv, int D, int max_seq_len) {
+  return pa_packed_prefill_workspace_bytes_for(num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len, 0);
 }
 
 int pa_packed_prefill(const void* q, const void* k, const void* v, long q_stride, long k_stride, long v_stride,
@@ -979,20 +988,17 @@ int pa_packed_prefill(const void* q, const void* k, const void* v, long q_stride
   if ((long)total_q * (Hq / Hkv) + num_seqs > 0x7fff0000L)
     return fail_arg("%s: %d rows of %d q heads per kv head exceed 2^31", who, total_q, Hq / Hkv);
   if ((long)total_q + total_k > 0x7fffffffL) return fail_arg("%s: %d query and %d key rows exceed 2^31 together", who, total_q, total_k);
-  // A window of all keys there are is none.  (Kept, its length behind a query that lies before its sequence's first key --
-  // fewer keys than queries -- would be a position past the smallest integer; the two row counts bound what is left.)
-  if (sliding_window >= total_k) sliding_window = 0;
   if (num_seqs == 0 || total_q == 0) return 0;
   if (!q || !cu_seqlens_q || !out || (total_k > 0 && (!k || !v)) || !cu_seqlens_k) return fail_arg("%s: null pointer argument", who);
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return fail_arg("%s: q, k, v and out must be 16-byte aligned", who);
   if (!aligned16(workspace)) return fail_arg("%s: workspace must be 16-byte aligned", who);
   PrefillParams p;
-  fill_packed_shape(p, num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len);
+  fill_packed_shape(p, num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len, sliding_window);
   p.q = q; p.k = k; p.v = v; p.out = out;
   p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.query_lens = query_lens; p.seq_lens = seq_lens;
   p.q_stride = q_stride; p.k_stride = k_stride; p.v_stride = v_stride;
   p.scale_log2e = scale * kLog2e;
-  p.sinks = sinks; p.window = sliding_window;
+  p.sinks = sinks;
   p.splits = 1;
   if (workspace) {
     const int forced = g_prefill_split.load();       // 1: the rule; 0: never; 2-16: that many shares

@@ -619,12 +619,12 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
             raise ValueError(f"out must be bfloat16 {(Nq, Hq, D)}")
     with _on(q.device):
         stream = _stream_ptr(q.device)
-        key = (S, Nq, Nk, Hq, Hkv, D, bound)
+        key = (S, Nq, Nk, Hq, Hkv, D, bound, win)
         need = _packed_need.get(key)
         if need is None:
             if len(_packed_need) >= 4096:
                 _packed_need.clear()
-            need = _packed_need[key] = int(lib.pa_packed_prefill_workspace_bytes(*key))
+            need = _packed_need[key] = int(lib.pa_packed_prefill_workspace_bytes_for(*key))
         if workspace is None:
             workspace = _workspace(q.device, need, stream) if need else None
         else:
@@ -640,9 +640,10 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
     return out
 
 
-def packed_prefill_workspace_bytes(num_seqs: int, total_q: int, total_k: int, Hq: int, Hkv: int, D: int, max_seq_len: int) -> int:
+def packed_prefill_workspace_bytes(num_seqs: int, total_q: int, total_k: int, Hq: int, Hkv: int, D: int, max_seq_len: int,
+                                   sliding_window=None) -> int:
     """Scratch bytes `packed_prefill` would use (0 for calls that take none)."""
-    return int(_lib.load().pa_packed_prefill_workspace_bytes(num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len))
+    return int(_lib.load().pa_packed_prefill_workspace_bytes_for(num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len, sliding_window or 0))
 
 
 def gather_kv(cache, block_tables, seq_lens, max_seq_len=None):

@@ -29,3 +29,18 @@ def test_a_window_of_all_rows_is_none(pa, rng, Hq, Hkv, D):  # noqa: F811
     want = pa.packed_prefill(q, k, v, cu, 0.1)
     for window in (sum(n), sum(n) + 1, 2 ** 31 - 1):
         assert torch.equal(pa.packed_prefill(q, k, v, cu, 0.1, sliding_window=window), want)
+
+
+@pytest.mark.parametrize("window", [50, 600, 1500, None])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (8, 2, 64), (3, 1, 64)])
+def test_chunks_behind_long_prefixes_in_the_shares_the_rule_gives(pa, rng, Hq, Hkv, D, window):  # noqa: F811
+    """The call's own scratch, and scratch of exactly the size asked for."""
+    qn, kn = [30, 1, 77, 100], [2100, 1500, 1300, 2600]
+    need = pa.packed_prefill_workspace_bytes(4, sum(qn), sum(kn), Hq, Hkv, D, max(kn), window)
+    assert need > 0 if window is None else window > 50 or need == 0
+    _, _, _, got = _run(pa, rng, qn, Hq, Hkv, D, kn=kn, window=window, max_seq_len=max(kn))
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    _run(pa, rng, qn, Hq, Hkv, D, kn=kn, window=window, max_seq_len=max(kn), workspace=ws)
+    if need:
+        with pytest.raises(ValueError):
+            _run(pa, rng, qn, Hq, Hkv, D, kn=kn, window=window, max_seq_len=max(kn), workspace=ws[:need - 16])

@@ -22,3 +22,26 @@ def test_rows_beyond_the_positions_of_32_bits(lib):
         return lib.pa_packed_prefill(P, P, P, 128, 128, 128, P, P, Z, Z, P, Z, 0, 2, nq, nk, 1, 1, 128, 0, 0.1, 1, Z, 0, Z)
     assert call((1 << 31) - (1 << 17), 1 << 17) == -1 and b"2^31 together" in lib.pa_last_error()
     assert call(0, 1 << 17) == 0
+
+
+# Without a device the library counts 256 compute units.
+def _shares(lib, S, nq, nk, Hq, Hkv, D, bound, window=0):
+    """Shares of a query tile's keys that a call asks scratch for (1: none)."""
+    n = lib.pa_packed_prefill_workspace_bytes_for(S, nq, nk, Hq, Hkv, D, bound, window)
+    per = nq * Hq * (D + 2) * 4
+    assert n % per == 0 and n // per != 1
+    return max(n // per, 1)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (64, 8, 64)])
+def test_shares_under_a_window_are_those_of_its_keys(lib, Hq, Hkv, D):
+    """Four chunks of 100 tokens behind some 3 000 keys: many keys in front split a tile, the few of a narrow window do not;
+    a window over all of them changes nothing."""
+    args = (4, 400, 12600, Hq, Hkv, D, 3200)
+    assert _shares(lib, *args) >= 4
+    for window in (1, 50, 128, 500):
+        assert _shares(lib, *args, window) == 1
+    assert _shares(lib, *args, 2000) <= 4
+    assert _shares(lib, *args, 12600) == _shares(lib, *args, 2 ** 31 - 1) == _shares(lib, *args)
+    assert lib.pa_packed_prefill_workspace_bytes(*args) == lib.pa_packed_prefill_workspace_bytes_for(*args, 0)
+    assert lib.pa_packed_prefill_workspace_bytes_for(*args, -1) == 0
