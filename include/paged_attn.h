@@ -242,7 +242,8 @@ int pa_prefill(const void* q, const void* k_cache, const void* v_cache,
  *   out           rows that belong to no sequence are left as they are
  *   sinks, sliding_window   as for pa_prefill, for both head dims; a window of total_k keys or more is none
  *   total_q + total_k  below 2^31
- *   max_seq_len   0, or a host-known upper bound of a sequence's keys (a hint: see the workspace)
+ *   max_seq_len   0, or a host-known upper bound of a sequence's keys (a hint: see the workspace; 0 counts as twice the
+ *                 mean of the sequences' rows)
  *   workspace     NULL, or pa_packed_prefill_workspace_bytes(...) bytes (16-byte aligned; 0 = none needed): with it, a
  *                 call of few queries over many keys splits the keys of a query tile over several workgroups and merges
  *                 their results in a second kernel.  ..._for answers for a call under a sliding window, which has fewer

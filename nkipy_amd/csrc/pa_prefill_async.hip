@@ -1422,10 +1422,15 @@ int prefill_packed_splits(const PrefillParams& p, int num_cus) {
   // 256 tokens behind 32 K 474 / 120 (8; with 4 137, with 16 133), 512 behind 4 K 74 / 47 (4; 2 54, 8 57), 64 behind 8 K 107 /
   // 32 (16), 8 x 64 behind 8 K 161 / 79 (4); 64 / 8 heads of 64: 512 behind 4 K 106 / 53 (4), 256 behind 32 K 817 / 162 (8).
   // A call that already has two workgroups for every three places is left alone (4 x 257-512 behind 4 K: 105 / 119 with two
-  // shares), and so are prompts with less than twice their length in front of them, which their own diagonal bounds
-  // (1 x 1 024: 28.5 / 35.5).
+  // shares), and so are sequences of one length with less than twice their queries in front of these, which their own
+  // diagonal bounds (1 x 1 024: 28.5 / 35.5).  The longest context against the mean of the queries: one long prompt among short
+  // ones counts as few queries over many keys, which for a device with room it is (2 048 tokens and seven times 16, us
+  // unsplit / as the rule has it: 7 / 1 heads of 128 52.8 / 33.1, 16 / 2 53.3 / 45.9, 7 / 1 of 64 33.6 / 25.1, 8 / 2 of 64 34.0 / 31.7).
   if (!packed_takes_groups(p) && p.D == HD) return 1;
-  const long bound = p.len_bound > 0 ? p.len_bound : p.total_k, mean = p.total_q / p.B;
+  // No bound given: taken as twice the mean of the contexts (as all rows of the batch, which only a single sequence can have, eight
+  // prompts of 300 tokens without a prefix counted as 2 400 keys over 300 queries and were split: 16 / 2 heads of 128
+  // 13.1 us unsplit, 34.8 in two shares; 7 / 1 heads 13.1 / 31.5 in four).
+  const long bound = p.len_bound > 0 ? p.len_bound : std::min<long>(p.total_k, 2L * (p.total_k / p.B + 1)), mean = p.total_q / p.B;
   if (bound < 3 * mean) return 1;
   const int mult = p.D == HD ? p.Hq / p.Hkv : 1, shift = p.D == HD ? 7 : 6;
   const long tiles = std::max(1L, (((long)mult * p.total_q) >> shift) + p.B / 2);      // about: the last tile of a sequence is half full

@@ -581,7 +581,7 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
     queries in front of it as well, and of as many behind those whose window it is in (their weight for it is 0, and
     0 x inf is not).
     max_seq_len: host-known upper bound of a sequence's keys; sizes the split of calls with few queries over many keys
-    (default Nk).  sinks [Hq] / sliding_window as in `decode`, the window counted back from each query.
+    (default: twice the mean of the sequences' rows).  sinks [Hq] / sliding_window as in `decode`, the window counted back from each query.
     """
     lib = _lib.load()
     qs, ks, vs = _token_rows("q", q), _token_rows("k", k), _token_rows("v", v)
@@ -609,7 +609,7 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
                 raise ValueError(f"{n} must be int32 [num_seqs]")
     if not (max_seq_len is None or int(max_seq_len) > 0):
         raise ValueError(f"max_seq_len {max_seq_len} must be positive")
-    bound = Nk if max_seq_len is None else min(int(max_seq_len), Nk)
+    bound = 0 if max_seq_len is None else min(int(max_seq_len), Nk)
     sinks, win = _check_variant(sinks, sliding_window, Hq, q)
     if out is None:
         out = torch.empty((Nq, Hq, D), dtype=torch.bfloat16, device=q.device)
@@ -642,7 +642,7 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
 
 def packed_prefill_workspace_bytes(num_seqs: int, total_q: int, total_k: int, Hq: int, Hkv: int, D: int, max_seq_len: int,
                                    sliding_window=None) -> int:
-    """Scratch bytes `packed_prefill` would use (0 for calls that take none)."""
+    """Scratch bytes `packed_prefill` would use (0 for calls that take none); max_seq_len 0: the call gives none."""
     return int(_lib.load().pa_packed_prefill_workspace_bytes_for(num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len, sliding_window or 0))
 
 

@@ -45,3 +45,14 @@ def test_shares_under_a_window_are_those_of_its_keys(lib, Hq, Hkv, D):
     assert _shares(lib, *args, 12600) == _shares(lib, *args, 2 ** 31 - 1) == _shares(lib, *args)
     assert lib.pa_packed_prefill_workspace_bytes(*args) == lib.pa_packed_prefill_workspace_bytes_for(*args, 0)
     assert lib.pa_packed_prefill_workspace_bytes_for(*args, -1) == 0
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (16, 2, 128), (7, 1, 128), (64, 8, 64), (8, 2, 64), (7, 1, 64)])
+def test_shares_of_a_call_without_a_bound(lib, Hq, Hkv, D):
+    """No bound on the contexts is not one context of all the batch's rows: prompts without a prefix stay whole, a few tokens
+    behind long contexts are split as with the bound."""
+    assert _shares(lib, 8, 2400, 2400, Hq, Hkv, D, 0) == 1
+    assert _shares(lib, 64, 64 * 64, 64 * 64, Hq, Hkv, D, 0) == 1
+    assert _shares(lib, 1, 1024, 1024, Hq, Hkv, D, 0) == 1
+    assert _shares(lib, 1, 64, 8192, Hq, Hkv, D, 0) == _shares(lib, 1, 64, 8192, Hq, Hkv, D, 8192) >= 8
+    assert _shares(lib, 2, 64, 16384, Hq, Hkv, D, 0) >= 4
