@@ -1434,14 +1434,25 @@ int prefill_packed_splits(const PrefillParams& p, int num_cus) {
   if (bound < 3 * mean) return 1;
   const int mult = p.D == HD ? p.Hq / p.Hkv : 1, shift = p.D == HD ? 7 : 6;
   const long tiles = std::max(1L, (((long)mult * p.total_q) >> shift) + p.B / 2);      // about: the last tile of a sequence is half full
-  const long wgs = tiles * packed_groups(p) * packed_heads_per_group(p, p.D == 64 ? d64_heads_per_wave(p) : 1), places = 2L * num_cus;
+  const int heads = p.D == 64 ? d64_heads_per_wave(p) : 1;
+  const long wgs = tiles * packed_groups(p) * packed_heads_per_group(p, heads), places = 2L * num_cus;
   // Under a sliding window a tile walks the window of its first query up to its last one, whatever lies in front of that; its
   // shares are shares of these keys.  32 / 8 heads of 128, 4 x 100 behind 3 K, us unsplit / in the five shares that its 3 200
   // keys without a window give: window 50 9.6 / 21.8, 128 12.2 / 26.9, 500 18.6 / 32.4; window 2 000, four shares, 49.7 / 36.2.
   long reach = bound;
   if (p.window > 0) reach = std::min<long>(reach, p.window + (p.D == HD ? 128 / mult + 1 : 64) + 63);
-  const long s = std::min((2 * places + wgs) / (2 * wgs), reach / (8 * 64));
-  return s < 2 ? 1 : (int)std::min(s, 16L);
+  // Head dim 64 with two q heads per wave: unsplit, a call of few workgroups runs with one (packed_form), twice as many of them,
+  // so that the two-thirds are counted on those, and two shares are as many workgroups as none and always behind (us,
+  // unsplit / 2 / 3 / 4 shares: 8 / 2 heads, 8 x 64 behind 1 000 21.1 / 26.3 / 22.7 / 21.5, 4 x 150 behind 2 K 36.1 / 40.9 / 33.0 /
+  // 29.4; 16 / 4, 8 x 64 behind 1 500 29.5 / 34.1 / 28.8 / 26.4; 64 / 8, 4 x 300 behind 3 K 112 / 121 / 111 / 117).  Where the
+  // unsplit workgroups already take a third of the places it takes four shares, of twelve key tiles, to pay (64 / 8:
+  // 2 x 256 behind 2 K 38.8 / 47.6 / 46.4 / 42.4, 1 x 512 behind 1 536 34.3 / 43.9 / 39.8 / 36.9, 2 x 200 under a window of 1 500 29.0 /
+  // 38.0 / 39.2 / 35.7; 4 x 100 behind 3 K 54.0 / 60.3 / - / 48.9, 1 x 512 behind 4 K 71.3 / 78.3 / 70.4 / 61.8).
+  const long whole = tiles * packed_groups(p) * packed_heads_per_group(p, 1);
+  const bool crowded = heads == 2 && 3 * whole >= places;
+  if ((2 * places + whole) / (2 * whole) < 2) return 1;
+  const long s = std::min((2 * places + wgs) / (2 * wgs), reach / ((crowded ? 12 : 8) * 64)), least = crowded ? 4 : heads == 2 ? 3 : 2;
+  return s < least ? 1 : (int)std::min(s, 16L);
 }
 
 hipError_t launch_prefill_packed(const PrefillParams& p0, hipStream_t s) {

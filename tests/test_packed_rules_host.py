@@ -56,3 +56,16 @@ def test_shares_of_a_call_without_a_bound(lib, Hq, Hkv, D):
     assert _shares(lib, 1, 1024, 1024, Hq, Hkv, D, 0) == 1
     assert _shares(lib, 1, 64, 8192, Hq, Hkv, D, 0) == _shares(lib, 1, 64, 8192, Hq, Hkv, D, 8192) >= 8
     assert _shares(lib, 2, 64, 16384, Hq, Hkv, D, 0) >= 4
+
+
+def test_shares_at_head_dim_64_are_more_workgroups_than_none(lib):
+    """A split wave takes two q heads where a whole one of a small call takes one: two shares are as many workgroups as none."""
+    for Hq, Hkv in ((64, 8), (8, 2), (16, 4), (32, 8), (2, 1)):
+        for S, T, ctx in ((4, 100, 3200), (8, 64, 1064), (8, 64, 1564), (2, 256, 2304), (1, 512, 2048), (1, 512, 4608), (4, 300, 3300), (1, 64, 8192)):
+            for window in (0, 700, 1500):
+                assert _shares(lib, S, S * T, S * ctx, Hq, Hkv, 64, ctx, window) != 2
+    assert _shares(lib, 8, 512, 8512, 8, 2, 64, 1064) == 1
+    assert _shares(lib, 2, 512, 4608, 64, 8, 64, 2304) == 1
+    assert _shares(lib, 1, 512, 4608, 64, 8, 64, 4608) == 4
+    assert _shares(lib, 1, 256, 33024, 64, 8, 64, 33024) == 8
+    assert _shares(lib, 4, 64, 2464, 7, 1, 64, 1232) == 2             # one q head per wave either way
