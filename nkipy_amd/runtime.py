@@ -82,7 +82,7 @@ class DeviceKernel:
     _OPS = {"decode": paged_attn.decode, "prefill": paged_attn.prefill,
             "blocksparse_prefill": paged_attn.blocksparse_prefill,
             "kv_write": paged_attn.kv_write, "qk_norm_rope_kv_write": paged_attn.qk_norm_rope_kv_write,
-            "o_proj": paged_attn.o_proj, "packed_prefill": paged_attn.packed_prefill}
+            "o_proj": paged_attn.o_proj, "packed_prefill": paged_attn.packed_prefill, "read_kv": paged_attn.read_kv}
 
     def __init__(self, fn, name, signature, static_kwargs):
         self.fn, self.name = fn, name
@@ -90,24 +90,33 @@ class DeviceKernel:
         self.static_kwargs = static_kwargs
         # in-place state: parameter names this op mutates and that the caller passed
         self.aliased = [k for k in _MUTATED.get(fn.__name__, ()) if k in signature]
-        # what the op returns by position ("output0"): the attention result, the transformed q, or nothing
+        # what the op returns by position ("output0", "output1"): shape and dtype of the attention result, of the transformed
+        # q, of the projection, of the rows read back (K, V), or nothing
         if fn is paged_attn.kv_write or (fn is paged_attn.qk_norm_rope_kv_write and "xq" not in signature):
-            self._result_like = None
-        else:
-            self._result_like = "xq" if fn is paged_attn.qk_norm_rope_kv_write else "q"
-        # shape and dtype of "output0"
-        self._result_sig = self.signature.get(self._result_like) if self._result_like else None
-        if fn is paged_attn.o_proj and "x" in signature and "o_weight" in signature:
+            self._results = []
+        elif fn is paged_attn.read_kv:
+            if static_kwargs.get("total_tokens") is None or "k_cache" not in signature:
+                raise ValueError("read_kv needs k_cache and total_tokens (rows of the results)")
+            row = (int(static_kwargs["total_tokens"]),) + signature["k_cache"][0][2:]
+            self._results = [(row, torch.bfloat16)] * 2
+        elif fn is paged_attn.o_proj and "x" in signature and "o_weight" in signature:
             (xs, xd), (ws, _) = signature["x"], signature["o_weight"]
             lead = xs[:-1] if xs[-1] == ws[0] else xs[:-2]          # x is [..., K] or [..., Hq, D]
-            self._result_like, self._result_sig = "x", (tuple(lead) + (ws[1],), xd)
-        self.output_names = (["output0"] if self._result_like else []) + list(self.aliased)
+            self._results = [(tuple(lead) + (ws[1],), xd)]
+        else:
+            self._results = [signature.get("xq" if fn is paged_attn.qk_norm_rope_kv_write else "q")]
+        self.output_names = [f"output{i}" for i in range(len(self._results))] + list(self.aliased)
         # names the caller uses for inputs: mutated parameters carry the alias suffix
         self.input_names = {(k + ALIAS_SUFFIX if k in self.aliased else k): k for k in signature}
 
+    @property
+    def _result_sig(self):
+        """Shape and dtype of "output0", None without one."""
+        return self._results[0] if self._results else None
+
     @classmethod
     def compile_and_load(cls, fn, name: str | None = None, **example_args) -> "DeviceKernel":
-        """fn: one of nkipy_amd.decode / prefill / blocksparse_prefill / packed_prefill / kv_write /
+        """fn: one of nkipy_amd.decode / prefill / blocksparse_prefill / packed_prefill / kv_write / read_kv /
         qk_norm_rope_kv_write / o_proj (or its name).  Tensor arguments (DeviceTensor or torch tensor), given
         under the op's parameter names, fix the expected shapes and dtypes; every other keyword
         (scale, partition_size, ...) becomes a static argument of the kernel."""
@@ -149,7 +158,7 @@ class DeviceKernel:
             assert tuple(t.shape) == shape, f"input {name!r}: shape {tuple(t.shape)} != {shape}"
             assert t.dtype == dtype, f"input {name!r}: dtype {t.dtype} != {dtype}"
             args[k] = t
-        out = None
+        given = [None] * len(self._results)
         if outputs is not None:
             for k in self.aliased:          # an alias output is the buffer that came in under the alias name
                 if k in outputs:
@@ -157,18 +166,23 @@ class DeviceKernel:
                     o = o.tensor if isinstance(o, DeviceTensor) else o
                     assert o.data_ptr() == args[k].data_ptr() and tuple(o.shape) == tuple(args[k].shape), \
                         f"output {k!r} must be the buffer passed as input {k + ALIAS_SUFFIX!r}"
-            if "output0" in outputs:
-                o = outputs["output0"]
-                out = o.tensor if isinstance(o, DeviceTensor) else o
-                qshape, qdtype = self._result_sig
-                assert tuple(out.shape) == qshape and out.dtype == qdtype, \
-                    f"output0 must be {qdtype} {qshape}"
-        if self._result_like is None:
+            for i, (want_shape, want_dtype) in enumerate(s for s in self._results if s is not None):
+                name = f"output{i}"
+                if name in outputs:
+                    o = outputs[name]
+                    given[i] = o.tensor if isinstance(o, DeviceTensor) else o
+                    assert tuple(given[i].shape) == tuple(want_shape) and given[i].dtype == want_dtype, \
+                        f"{name} must be {want_dtype} {tuple(want_shape)}"
+        if not self._results:
             self.fn(**args, **self.static_kwargs)
-            res = None
+            res = []
+        elif len(self._results) == 1:
+            res = [self.fn(**args, **self.static_kwargs, out=given[0])]
         else:
-            res = self.fn(**args, **self.static_kwargs, out=out)
+            if any(g is not None for g in given):      # both or neither reach the op: a result the caller gives no room for is made here
+                given = [torch.empty(s, dtype=d, device=args["k_cache"].device) if g is None else g for g, (s, d) in zip(given, self._results)]
+            res = list(self.fn(**args, **self.static_kwargs, out=tuple(given) if given[0] is not None else None))
         if outputs is None:
-            ret = ([DeviceTensor(res)] if self._result_like else []) + [DeviceTensor(args[k]) for k in self.aliased]
+            ret = [DeviceTensor(r) for r in res] + [DeviceTensor(args[k]) for k in self.aliased]
             return ret[0] if len(ret) == 1 else (tuple(ret) if ret else None)
         return None
