@@ -79,8 +79,9 @@ def blocksparse_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale
 # operator cannot be optional.
 @torch.library.custom_op(f"{_NS}::paged_kv_write", mutates_args=("k_cache", "v_cache"), device_types="cuda")
 def paged_kv_write(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-                   block_tables: torch.Tensor, seq_lens: torch.Tensor, query_lens: torch.Tensor) -> None:
-    paged_attn.kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens)
+                   block_tables: torch.Tensor, seq_lens: torch.Tensor, query_lens: torch.Tensor,
+                   cu_seqlens: Optional[torch.Tensor] = None) -> None:
+    paged_attn.kv_write(k_new, v_new, k_cache, v_cache, block_tables, seq_lens, query_lens, cu_seqlens=cu_seqlens)
 
 
 @torch.library.custom_op(f"{_NS}::paged_kv_write_fp8", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"),

@@ -67,3 +67,27 @@ def test_a_chunk_by_names():
     att = {"q": q, "k": k2, "v": v2, "cu_seqlens": cu, "cu_seqlens_k": cu_ctx}
     out = DeviceKernel.compile_and_load("packed_prefill", scale=0.125, max_seq_len=51, **att)(inputs=att)
     assert torch.equal(out.torch(), pa.packed_prefill(q, *want, cu, 0.125, cu_seqlens_k=cu_ctx, max_seq_len=51))
+
+
+def test_packed_writes_are_in_the_dispatcher():
+    import nkipy_amd.torch_ops  # noqa: F401
+    for name in ("paged_kv_write", "paged_kv_write_int8"):
+        assert "Tensor? cu_seqlens=None" in str(getattr(torch.ops.nkipy_amd, name).default._schema)
+
+
+@pytest.mark.gpu
+def test_a_packed_write_through_the_dispatcher():
+    """bfloat16 pools: packed rows, slices of a wider tensor, as the Python call writes them."""
+    import nkipy_amd as pa
+    import nkipy_amd.torch_ops  # noqa: F401
+    rng = np.random.default_rng(4)
+    Hkv, D, bs, n = 2, 128, 32, [37, 0, 50]
+    wide = torch.from_numpy(rng.standard_normal((87, 3 * Hkv, D)).astype(np.float32)).cuda().to(torch.bfloat16)
+    k, v = wide[:, :Hkv], wide[:, 2 * Hkv:]
+    tables, lens, cu = _i32([[0, 1], [2, 3], [4, 5]], "cuda"), _i32([40, 3, 50], "cuda"), _i32([0, 37, 37, 87], "cuda")
+    pools = [torch.zeros((6, bs, Hkv, D), dtype=torch.bfloat16, device="cuda") for _ in range(4)]
+    torch.ops.nkipy_amd.paged_kv_write(k, v, pools[0], pools[1], tables, lens, _i32(n, "cuda"), cu)
+    pa.kv_write(k, v, pools[2], pools[3], tables, lens, _i32(n, "cuda"), cu_seqlens=cu)
+    assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3]) and bool((pools[0] != 0).any())
+    k2, v2 = pa.read_kv(pools[0], pools[1], tables, _i32([40, 0, 50], "cuda"), _i32([0, 40, 40, 90], "cuda"), 90)
+    assert torch.equal(k2[3:40], k[:37]) and torch.equal(v2[40:], v[37:])
