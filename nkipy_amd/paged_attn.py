@@ -180,6 +180,7 @@ def _check_variant(sinks, sliding_window, Hq, ref):
     variant (examples/models/gpt_oss/kernels/attention.py:117-148).  Returns (sinks_f32 or None, window int)."""
     win = 0 if sliding_window is None else int(sliding_window)
     _check(win >= 0 and (sliding_window is None or win >= 1), "sliding_window must be None or >= 1")
+    win = min(win, 0x7fffffff)      # (the C argument is 32 bits wide: 2^32 + 5 arrived as a window of five keys)
     if sinks is not None:
         _need_device("sinks", sinks)
         _check(sinks.shape == (Hq,), f"sinks must have one logit per q head ([{Hq}])")
@@ -643,7 +644,8 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
 def packed_prefill_workspace_bytes(num_seqs: int, total_q: int, total_k: int, Hq: int, Hkv: int, D: int, max_seq_len: int,
                                    sliding_window=None) -> int:
     """Scratch bytes `packed_prefill` would use (0 for calls that take none); max_seq_len 0: the call gives none."""
-    return int(_lib.load().pa_packed_prefill_workspace_bytes_for(num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len, sliding_window or 0))
+    return int(_lib.load().pa_packed_prefill_workspace_bytes_for(num_seqs, total_q, total_k, Hq, Hkv, D, max_seq_len,
+                                                                 min(sliding_window or 0, 0x7fffffff)))
 
 
 def gather_kv(cache, block_tables, seq_lens, max_seq_len=None):

@@ -44,3 +44,19 @@ def test_chunks_behind_long_prefixes_in_the_shares_the_rule_gives(pa, rng, Hq, H
     if need:
         with pytest.raises(ValueError):
             _run(pa, rng, qn, Hq, Hkv, D, kn=kn, window=window, max_seq_len=max(kn), workspace=ws[:need - 16])
+
+
+def test_a_window_past_32_bits_is_none(pa, rng):  # noqa: F811
+    """Every call that takes a window, over contexts longer than what is left of it in 32 bits.  Either result is off by the
+    rounding of its probabilities and its own, 2^-8 of max |v| each."""
+    Hq, Hkv, D, bs, n = 8, 2, 128, 32, 150
+    q, k, v = (bf16(O.round_to_bf16(rng.standard_normal((n, h, D)).astype(np.float32))) for h in (Hq, Hkv, Hkv))
+    cu, ln = dev(np.asarray([0, n], np.int32)), dev(np.asarray([n], np.int32))
+    tables = dev(rng.permutation(5).astype(np.int32)[None])
+    kc, vc = (torch.zeros((5, bs, Hkv, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pa.kv_write(k, v, kc, vc, tables, ln, ln, cu_seqlens=cu)
+    four = dev(np.asarray([4], np.int32))
+    for call in (lambda w: pa.packed_prefill(q, k, v, cu, 0.1, sliding_window=w), lambda w: pa.decode(q[-1:], kc, vc, tables, ln, 0.1, sliding_window=w),
+                 lambda w: pa.prefill(q[None], kc, vc, tables, ln, ln, 0.1, sliding_window=w),
+                 lambda w: pa.verify(q[None, -4:].contiguous(), kc, vc, tables, ln, four, 0.1, sliding_window=w)):
+        assert (call(2 ** 32 + 5).float() - call(None).float()).abs().max() <= 4 * 2.0 ** -8 * v.float().abs().max()

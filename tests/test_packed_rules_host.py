@@ -69,3 +69,14 @@ def test_shares_at_head_dim_64_are_more_workgroups_than_none(lib):
     assert _shares(lib, 1, 512, 4608, 64, 8, 64, 4608) == 4
     assert _shares(lib, 1, 256, 33024, 64, 8, 64, 33024) == 8
     assert _shares(lib, 4, 64, 2464, 7, 1, 64, 1232) == 2             # one q head per wave either way
+
+
+def test_a_window_past_32_bits_is_no_short_one():
+    from nkipy_amd import paged_attn
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 40):
+        assert paged_attn._check_variant(None, window, 4, None) == (None, 2 ** 31 - 1)
+    assert paged_attn._check_variant(None, 5, 4, None) == (None, 5) and paged_attn._check_variant(None, None, 4, None) == (None, 0)
+    with pytest.raises(ValueError):
+        paged_attn._check_variant(None, -5, 4, None)
+    assert paged_attn.packed_prefill_workspace_bytes(4, 400, 12600, 32, 8, 128, 3200, 2 ** 32 + 5) == \
+        paged_attn.packed_prefill_workspace_bytes(4, 400, 12600, 32, 8, 128, 3200)
