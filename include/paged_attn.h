@@ -121,7 +121,8 @@ size_t pa_decode_workspace_bytes_for(int B, int Hq, int Hkv, int D, int block_si
  * max_seq_len: upper bound of seq_lens (sizes the grid and picks the kernel; 0 =
  * max_blocks_per_seq * block_size).  seq_lens[b] == 0 yields zeros.
  * q_dtype / kv_dtype: (F32, F32), (BF16, BF16), (BF16, FP8_E4M3FN) or, on the MFMA kernels' shapes only,
- *   (BF16, INT8).
+ *   (BF16, INT8): a query row then goes in as 16-bit integers, elements of at least 2^-6 of its largest as they are,
+ *   smaller ones rounded to 2^-15 of that at most.
  * sinks: NULL, or [Hq] float32 per-head logits that join every softmax as one more column and
  *   are dropped afterwards (examples/models/gpt_oss/kernels/attention.py:137-148): they only
  *   enlarge the denominator.  sliding_window: 0, or W >= 1: the query at position p sees the W

@@ -413,12 +413,14 @@ struct DecodeWave {
     }
   }
 
-  // int8: the row's values become 16-bit integers under a scale of their own, absmax / 32 512, in two limbs of 8 bits (256
-  // high + low, both signed): the score product is then the integer matrix instruction's on the codes as they lie in
-  // memory, exact, where a conversion to bf16 costs three vector instructions for two codes (64 / 8 heads of 128, 64
-  // sequences of 1 024-32 768 tokens: 203 -> 194 us, 6.0 TB/s; 64 / 8 heads of 64, 64 of 512-8 192: 80 -> 75.5, now 70.6).  An element is rounded at
-  // most half a step, 2^-16 of the row's largest (2^-121 where that is less: steps below 2^-120 have no reciprocal); a bf16 value at least 2^-8 of the largest is not rounded at all.  Slot
-  // limb * KLD + s holds limb 0 (high) or 1 (low) of the 16 elements that lane (g, .) has of step s.  A row with an
+  // int8: the row's values become 16-bit integers under a step of their own, in two limbs of 8 bits (256 high + low, both
+  // signed): the score product is then the integer matrix instruction's on the codes as they lie in memory, exact, where a
+  // conversion to bf16 costs three vector instructions for two codes (64 / 8 heads of 128, 64 sequences of
+  // 1 024-32 768 tokens: 203 -> 194 us, 6.0 TB/s; 64 / 8 heads of 64, 64 of 512-8 192: 80 -> 75.5, now 70.6).  The step is 2^-14 of the
+  // power of two below the row's largest element, so an element at least 2^-6 of the largest goes in without rounding (a bf16 value
+  // has 8 bits); a smaller one is off by at most half a step, 2^-16 to 2^-15 of the largest (2^-121 where that is less: steps
+  // below 2^-120 have no inverse).  One significand, 255 / 128, would pass the limbs' 127 x 256 + 127: it takes the next power.
+  // Slot limb * KLD + s holds limb 0 (high) or 1 (low) of the 16 elements that lane (g, .) has of step s.  A row with an
   // infinity or a NaN gets the scale NaN.
   __device__ __forceinline__ void q_limbs(uint4 (&qraw)[KSTEPS], int rg) {
     uint4 hq[KLD], lq[KLD];
@@ -430,11 +432,9 @@ struct DecodeWave {
       for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));      // (orders as the magnitudes do, a NaN above infinity)
     }
     top = over_g(top, [](uint32_t a, uint32_t b) __attribute__((always_inline)) { return max(a, b); });
-    // (Reciprocals within an ulp do: absmax x inv rounds to 32 512 all the same, and the scale is inv's own.  The reciprocal
-    // of a number past 2^126 would be below the smallest normal one, which the instruction gives as zero: it is taken of
-    // 2^-20 times the number.)
-    const float inv = fminf(32512.f * 0x1p-20f * __builtin_amdgcn_rcpf(0x1p-20f * __uint_as_float(top << 16)), 0x1p+120f);
-    q_scale[I8 ? rg : 0] = top >= 0x7f80u ? __uint_as_float(0x7fc00000u) : p.scale_log2e * __builtin_amdgcn_rcpf(inv);
+    const uint32_t e = max((top + 1) >> 7, 21u);         // exponent field of that power of two
+    const float inv = __uint_as_float((268 - e) << 23);
+    q_scale[I8 ? rg : 0] = top >= 0x7f80u ? __uint_as_float(0x7fc00000u) : p.scale_log2e * __uint_as_float((e - 14) << 23);
 #pragma unroll
     for (int s = 0; s < KLD; ++s) {
       uint32_t hi[4], lo[4];

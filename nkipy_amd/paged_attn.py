@@ -296,6 +296,8 @@ def decode(q, k_cache, v_cache, block_tables, seq_lens, scale, *, k_scale=None, 
     in q's dtype, or float8_e4m3fn / uint8 codes with k_scale/v_scale [num_blocks, Hkv]
     float32, or int8 codes with k_scale/v_scale [num_blocks, Hkv, block_size] (one scale per token and kv head, as
     `kv_write` leaves them; head_dim 64 or 128, a power-of-two block size >= 16); block_tables int32 [B, max_blocks]; seq_lens int32 [B].
+    Over int8 pools a query row goes into the score product as 16-bit integers: elements of at least 2^-6 of the row's
+    largest as they are, smaller ones rounded to 2^-15 of it at most; the products with the codes are exact.
     max_seq_len: host-known upper bound of seq_lens (sizes the split-K grid
     without a device sync; default = table capacity).
     sinks [Hq]: per-head logits that join the softmax as one more column and carry no value;
