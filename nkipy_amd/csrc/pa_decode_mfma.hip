@@ -1535,11 +1535,14 @@ __global__ __launch_bounds__(256) void decode_balanced_reduce_kernel(DecodeParam
 // XCD, next to each other, where the units of such slots fill the eight XCDs evenly.  us per call, one by one / together: 32 / 8 heads of
 // 128, 16 sequences of 500-1 024, T = 8, int8 17.4 / 16.9, bf16 22.0 / 17.8; 1 of 4 096, T = 8, int8 15.9 / 15.1, fp8 14.8 / 13.9;
 // 64 / 8 heads of 64, 16 of 500-1 024, T = 4, int8 14.8 / 13.7, bf16 13.8 / 12.1.  Calls of fewer than 128 workgroups are left alone
-// (64 of them: 1 of 1 024, T = 4, 8.8 / 9.1; 1 of 4 096, T = 1, 10.8 / 11.0).
+// (64 of them: 1 of 1 024, T = 4, 8.8 / 9.1; 1 of 4 096, T = 1, 10.8 / 11.0), and so are groups of more than eight slots where not all
+// workgroups are on the device at once (two per CU): an XCD then has a few large groups of unlike lengths, and the longest
+// ones decide (32 / 2 heads of 128, T = 16, bf16 / fp8 pools: 32 of 300-600 56.4 / 61.6, 54.2 / 57.2; 18 of 300-600 36.8 /
+// 39.9, 35.6 / 37.4; 24 of 300-600 44.9 / 47.5, 42.4 / 44.8; groups of up to eight gain there, 32 / 8 heads, T = 8, 48 of 200-400, bf16 28.9 / 25.8).
 static int line_group_of(const DecodeParams& p, int slots, int row_bytes) {
   const int heads = std::max(1, 128 / row_bytes), g = slots / p.Hkv * heads;
   const long workgroups = (long)slots * p.num_partitions * p.B;
-  if (!p.head_major || g <= 1 || p.Hkv % heads || workgroups < 128 || workgroups > 0x7fffffffL) return 1;
+  if (!p.head_major || g <= 1 || p.Hkv % heads || workgroups < 128 || workgroups > (g > 8 ? 512 : 0x7fffffffL)) return 1;
   return workgroups / g % 8 == 0 ? g : 1;
 }
 template <int D, int KV>
