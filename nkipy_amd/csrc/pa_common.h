@@ -291,6 +291,7 @@ struct DecodeParams {
   float scale_log2e;
   int head_major;           // fixed-partition grid order: kv head fastest (1) or partition fastest (0)
   int line_group;           // ... and how many neighbouring head slots share an XCD (set by the launcher)
+  FastDiv by_line_group, by_groups, by_parts;   // line_group, head slots / line_group, num_partitions
   int bal_hsw, bal_ns, bal_gv;  // balanced schedule: head slots and chunks per workgroup, total chunks
   int bal_lockstep;         // keep the head waves of a workgroup on the same tile with a barrier
   QTransform qt;            // balanced schedule only: Q rows are normed and rotated as they are loaded

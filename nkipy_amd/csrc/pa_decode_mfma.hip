@@ -1065,11 +1065,11 @@ __global__ __launch_bounds__(NW * 64, NW > 4 ? 1 : 2) void decode_mfma_kernel(De
   int part = p.head_major ? blockIdx.y : blockIdx.x, b = blockIdx.z;
   int hidx = p.head_major ? blockIdx.x : blockIdx.y;
   if (p.line_group > 1) {      // (see line_group_of; consecutive workgroups go to consecutive XCDs)
-    const int id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z), k = id >> 3, turn = k / p.line_group;
-    const int unit = 8 * turn + (id & 7), groups = gridDim.x / p.line_group, rest = unit / groups;
-    hidx = (unit - rest * groups) * p.line_group + k - turn * p.line_group;
-    b = rest / gridDim.y;
-    part = rest - b * gridDim.y;
+    const int id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z), k = id >> 3, turn = p.by_line_group.quot(k);
+    const int unit = 8 * turn + (id & 7), rest = p.by_groups.quot(unit);
+    hidx = (unit - rest * (int)p.by_groups.d) * p.line_group + k - turn * p.line_group;
+    b = p.by_parts.quot(rest);
+    part = rest - b * (int)p.by_parts.d;
   }
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -1551,6 +1551,7 @@ hipError_t launch_typed(const DecodeParams& p0, int waves, hipStream_t s) {
   const int n_rep = p.Hq / p.Hkv;
   const int slots = head_slots_of(p);                  // Hkv x 16-row groups of a kv head's rows
   p.line_group = line_group_of(p, slots, KV == KV_BF16 ? 2 * D : D);
+  p.by_line_group.set(p.line_group); p.by_groups.set(slots / p.line_group); p.by_parts.set(p.num_partitions);
   dim3 grid(p.num_partitions, slots, p.B);
   if (p.head_major) grid = dim3(slots, p.num_partitions, p.B);
   if (p.query_lens) {      // multi-token rows: the four-wave form
