@@ -241,6 +241,7 @@ int pa_prefill(const void* q, const void* k_cache, const void* v_cache,
  *   query t of a sequence of n queries and c keys sees keys j <= c - n + t: the last query sees them all; a query
  *                 that sees no key (c < n) gets zeros
  *   out           rows that belong to no sequence are left as they are
+ *   infinities and NaN in k and v reach the queries that see them (those of v in their own columns) and no others
  *   sinks, sliding_window   as for pa_prefill, for both head dims; a window of total_k keys or more is none
  *   total_q + total_k  below 2^31
  *   max_seq_len   0, or a host-known upper bound of a sequence's keys (a hint: see the workspace; 0 counts as twice the

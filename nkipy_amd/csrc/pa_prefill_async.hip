@@ -1065,10 +1065,121 @@ void prefill_async_kernel(PrefillParams p) {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run[j]), __float_as_uint(l_run[j]), false, false);
     l_run[j] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
   }
+  // Packed form: a masked weight is 0, and 0 times a value that is no number is none: a V row with an infinity or a NaN has
+  // spoiled the rows of the tiles that hold it, whether they see it or not.  Nothing on the way looks for it (a check of the fragments
+  // of masked tiles would be a fourth of their vector instructions); here a row's result is asked whether it is finite, one
+  // instruction per two elements (nothing on short prompts, 0.5 % on long ones), and a row that is not, and whose tiles hold such
+  // a value behind its mask, in a column where the keys it sees next to that have none, is computed again from the keys it
+  // sees alone (`again`): one such value in the middle of 8 192 tokens, 32 / 8 heads of 128, makes 0.55 ms 0.99, nothing but such values 1.27.
+  typedef __bf16 bf16_pair __attribute__((ext_vector_type(2)));
+  float spoilt[QH];                              // 0, or no number if the row's result holds one that is none
+#pragma unroll
+  for (int j = 0; j < QH; ++j) spoilt[j] = 0.f;
+  auto again = [&](int j) __attribute__((always_inline)) {
+    if constexpr (PACKED) {
+      const unsigned long long both = __ballot(qvalid && spoilt[j] != 0.f);
+      uint32_t rows = (uint32_t)both | (uint32_t)(both >> 32);
+      if (rows == 0) return;
+      wait_vmcnt<0>();                           // the rows' stores are through before they are stored again
+      constexpr int LPR = DH / 8;                // lanes per row of values, 16 bytes each
+      // keys in the tiles this wave has worked on
+      const int t_lo = max(kt_begin, win > 0 ? max(prefix + wq_lo - win + 1, 0) / BN : 0) * BN;
+      const int t_hi = min(min(ntiles, max(prefix + wq_hi, 0) / BN + 1) * BN, ctx);
+      const char* krows = kbase + (PAIR && !solo ? par * 2 * DH : 0);
+      const char* vrows = vbase + (PAIR && !solo ? par * 2 * DH : 0);
+      while (rows) {
+        const int r = __builtin_ctz(rows);
+        rows &= rows - 1;
+        auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, r); };
+        const int last = of(qlim), first = win > 0 ? max(last - win + 1, 0) : 0;      // the keys it sees
+        const float l = __int_as_float(of(__float_as_int(l_run[j]))), m = __int_as_float(of(__float_as_int(m_ref[j])));
+        if (!(l < INFINITY)) continue;           // its scores are no numbers
+        uint32_t seen = 0, hidden = 0;           // of this lane's eight columns, those with a value that is no number
+        auto scan = [&](int from, int to) __attribute__((always_inline)) {
+#pragma unroll 1
+          for (int k0 = from; k0 < to; k0 += 64 / LPR) {
+            const int key = k0 + lane / LPR;
+            if (key >= to) continue;
+            const uint4 v = *(const uint4*)(vrows + key * v_row_bytes + (lane % LPR) * 16);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t found = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t top = (w[i] & 0x7f807f80u) + 0x00800080u;      // carries where an exponent is all ones
+              found |= ((top >> 15) & 1u) << (2 * i) | (top >> 31) << (2 * i + 1);
+            }
+            if (key < first || key > last) hidden |= found;
+            else seen |= found;
+          }
+        };
+        scan(t_lo, min(first, t_hi));
+        scan(max(max(first, t_lo), last - 63), t_hi);
+#pragma unroll
+        for (int off = LPR; off < 64; off <<= 1) {
+          seen |= (uint32_t)__shfl_xor((int)seen, off, 64);
+          hidden |= (uint32_t)__shfl_xor((int)hidden, off, 64);
+        }
+        if (__ballot((hidden & ~seen) != 0) == 0) continue;      // what it sees is no number
+        const long row = token_row(of(qrow));
+        const int head = of(hq_l) + j;
+        const uint4* qp = (const uint4*)((const uint16_t*)p.q + row * p.q_stride + (long)head * DH);
+        float acc[DH / 64];
+#pragma unroll
+        for (int i = 0; i < DH / 64; ++i) acc[i] = 0.f;
+        const int stop = min(last + 1, SPLIT ? ntiles * BN : last + 1);
+#pragma unroll 1
+        for (int k0 = max(first, SPLIT ? kt_begin * BN : 0); k0 < stop; k0 += 64) {
+          // a key per lane, then every lane its elements of each key's values
+          const int key = min(k0 + lane, stop - 1);
+          float dot = 0.f;
+#pragma unroll 4
+          for (int c = 0; c < DH / 8; ++c) {
+            const uint4 a = qp[c], b = *(const uint4*)(krows + key * kv_row_bytes + 16 * c);
+            const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              dot = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), dot);
+              dot = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), dot);
+            }
+          }
+          const float w = k0 + lane < stop ? __builtin_amdgcn_exp2f(fmaf(dot, sc, -m)) : 0.f;
+#pragma unroll 8
+          for (int i = 0; i < 64; ++i) {           // (past the end the last key again, which it sees, with no weight)
+            const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), i));
+            const char* vp = vrows + min(k0 + i, stop - 1) * v_row_bytes + lane * (DH / 32);
+            if constexpr (DH == 128) {
+              const uint32_t v = *(const uint32_t*)vp;
+              acc[0] = fmaf(wi, __uint_as_float(v << 16), acc[0]);
+              acc[DH / 64 - 1] = fmaf(wi, __uint_as_float(v & 0xffff0000u), acc[DH / 64 - 1]);
+            } else {
+              acc[0] = fmaf(wi, __uint_as_float((uint32_t)*(const uint16_t*)vp << 16), acc[0]);
+            }
+          }
+        }
+        if (SPLIT) {
+          float* po = p.ws_o + ((row * p.Hq + head) * p.splits + part) * DH + lane * (DH / 64);
+#pragma unroll
+          for (int i = 0; i < DH / 64; ++i) po[i] = acc[i];
+        } else {
+          const float inv = l > 0.f ? 1.f / l : 0.f;
+          uint16_t* po = out + row * q_row_stride + (long)head * DH + lane * (DH / 64);
+          const uint32_t w = pack_bf16x2(acc[0] * inv, acc[DH / 64 - 1] * inv);
+          if constexpr (DH == 128) *(uint32_t*)po = w;
+          else *po = (uint16_t)w;
+        }
+      }
+    }
+  };
   if (SPLIT) {     // partial result relative to m_ref; the sink and the division belong to the merge
     if (qvalid) {
 #pragma unroll
       for (int j = 0; j < QH; ++j) {
+        if (PACKED) {
+#pragma unroll
+          for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) spoilt[j] = fmaf(oacc[j][c][i], 0.f, spoilt[j]);
+        }
         float* po = p.ws_o + ((row_g + j) * p.splits + part) * DH;
 #pragma unroll
         for (int c = 0; c < VC; ++c)
@@ -1080,6 +1191,8 @@ void prefill_async_kernel(PrefillParams p) {
           *(float2*)(p.ws_ml + ((row_g + j) * p.splits + part) * 2) = make_float2(slack[j] == -INFINITY ? -INFINITY : m_ref[j], l_run[j]);
       }
     }
+#pragma unroll
+    for (int j = 0; j < QH; ++j) again(j);
     return;
   }
   // attention sink: a per-head logit that joins the softmax as one more column with no value
@@ -1103,6 +1216,10 @@ void prefill_async_kernel(PrefillParams p) {
         const int d = 32 * c + 8 * i4 + 4 * h;
         const uint32_t w0 = qvalid ? pack_bf16x2(oacc[hj][c][4 * i4] * inv, oacc[hj][c][4 * i4 + 1] * inv) : 0u;
         const uint32_t w1 = qvalid ? pack_bf16x2(oacc[hj][c][4 * i4 + 2] * inv, oacc[hj][c][4 * i4 + 3] * inv) : 0u;
+        if (PACKED) {
+          spoilt[hj] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16_pair, w0), __builtin_bit_cast(bf16_pair, 0u), spoilt[hj], false);
+          spoilt[hj] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16_pair, w1), __builtin_bit_cast(bf16_pair, 0u), spoilt[hj], false);
+        }
         *(uint2*)(patch + n * OROW_B + 2 * d) = make_uint2(w0, w1);
       }
     // the wave reads back what its own lanes wrote: no barrier, the compiler orders the LDS accesses
@@ -1116,6 +1233,8 @@ void prefill_async_kernel(PrefillParams p) {
                      make_uint4(lo.x, lo.y, hi.x, hi.y));
     }
   }
+#pragma unroll
+  for (int j = 0; j < QH; ++j) again(j);
 }
 
 // Merge of the split form: one thread per (query row, 4 consecutive d); rows past query_lens become zeros.

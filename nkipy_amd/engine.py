@@ -277,8 +277,7 @@ class PagedAttention:
     query_lens[b] rows; idle slots 0).  `attend` applies the optional QK RMSNorm + RoPE, writes K/V
     into the layer's pool and runs the prefill / verify kernel (T > 1) or the decode kernel
     (T == 1); over an int8 cache a long chunk reads the contexts back as bfloat16 rows (`read_kv`) and attends to those
-    (`packed_prefill`, which expects finite rows: a row of the cache that held an infinity or a NaN reads back as NaN).
-    Returns [max_seqs, T, Hq, D] (a preallocated buffer, overwritten by the next step of
+    (`packed_prefill`; a row of the cache that held an infinity or a NaN reads back as NaN).  Returns [max_seqs, T, Hq, D] (a preallocated buffer, overwritten by the next step of
     the same T), or, when the layer was given `o_weight`, the output projection of it, [max_seqs, T, hidden].
 
     `attend` makes no host synchronisation and, after the first call of a given T, no allocation (but for the rows that a

@@ -580,9 +580,8 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
     seq_lens[i] keys (rows laid out with room to spare); the other query rows are padding, zero in the result, and the
     other keys are never read.  A query that sees no key gets zeros; rows that belong to no sequence are left as they
     are (whatever the memory held in a result allocated here).
-    K and V rows are expected to be finite: a V row with an infinity or a NaN can reach the rows of up to 95
-    queries in front of it as well, and of as many behind those whose window it is in (their weight for it is 0, and
-    0 x inf is not).
+    An infinity or a NaN in a row reaches the queries that see it (a V row's in its own columns) and no others; the rows
+    whose tiles it spoilt are computed again, which costs such calls up to twice the time and more.
     max_seq_len: host-known upper bound of a sequence's keys; sizes the split of calls with few queries over many keys
     (default: twice the mean of the sequences' rows).  sinks [Hq] / sliding_window as in `decode`, the window counted back from each query.
     """
