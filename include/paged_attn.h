@@ -244,8 +244,8 @@ int pa_prefill(const void* q, const void* k_cache, const void* v_cache,
  *   infinities and NaN in k and v reach the queries that see them (those of v in their own columns) and no others
  *   sinks, sliding_window   as for pa_prefill, for both head dims; a window of total_k keys or more is none
  *   total_q + total_k  below 2^31
- *   max_seq_len   0, or a host-known upper bound of a sequence's keys (a hint: see the workspace; 0 counts as twice the
- *                 mean of the sequences' rows)
+ *   max_seq_len   0, or a host-known upper bound of a sequence's keys (a hint: see the workspace; 0 counts as
+ *                 total_k where that is at least 3 total_q, else as twice the mean of the sequences' keys)
  *   workspace     NULL, or pa_packed_prefill_workspace_bytes(...) bytes (16-byte aligned; 0 = none needed): with it, a
  *                 call of few queries over many keys splits the keys of a query tile over several workgroups and merges
  *                 their results in a second kernel.  ..._for answers for a call under a sliding window, which has fewer

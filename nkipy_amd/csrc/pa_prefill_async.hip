@@ -1546,10 +1546,12 @@ int prefill_packed_splits(const PrefillParams& p, int num_cus) {
   // ones counts as few queries over many keys, which for a device with room it is (2 048 tokens and seven times 16, us
   // unsplit / as the rule has it: 7 / 1 heads of 128 52.8 / 33.1, 16 / 2 53.3 / 45.9, 7 / 1 of 64 33.6 / 25.1, 8 / 2 of 64 34.0 / 31.7).
   if (!packed_takes_groups(p) && p.D == HD) return 1;
-  // No bound given: taken as twice the mean of the contexts (as all rows of the batch, which only a single sequence can have, eight
-  // prompts of 300 tokens without a prefix counted as 2 400 keys over 300 queries and were split: 16 / 2 heads of 128
-  // 13.1 us unsplit, 34.8 in two shares; 7 / 1 heads 13.1 / 31.5 in four).
-  const long bound = p.len_bound > 0 ? p.len_bound : std::min<long>(p.total_k, 2L * (p.total_k / p.B + 1)), mean = p.total_q / p.B;
+  // No bound given: the longest context may be one of all the batch's rows (a single sequence, or one among empty ones), and is
+  // taken as that where there are three times as many keys as queries.  Otherwise it is taken as twice the mean: as 2 400 keys
+  // over 300 queries eight prompts of 300 tokens without a prefix were split (16 / 2 heads of 128 13.1 us unsplit, 34.8 in two
+  // shares; 7 / 1 heads 13.1 / 31.5 in four).
+  const long mean = p.total_q / p.B;
+  const long bound = p.len_bound > 0 ? p.len_bound : p.total_k >= 3L * p.total_q ? p.total_k : std::min<long>(p.total_k, 2L * (p.total_k / p.B + 1));
   if (bound < 3 * mean) return 1;
   const int mult = p.D == HD ? p.Hq / p.Hkv : 1, shift = p.D == HD ? 7 : 6;
   const long tiles = std::max(1L, (((long)mult * p.total_q) >> shift) + p.B / 2);      // about: the last tile of a sequence is half full

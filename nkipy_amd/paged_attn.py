@@ -583,7 +583,8 @@ def packed_prefill(q, k, v, cu_seqlens, scale, *, cu_seqlens_k=None, query_lens=
     An infinity or a NaN in a row reaches the queries that see it (a V row's in its own columns) and no others; the rows
     whose tiles it spoilt are computed again, which costs such calls up to twice the time and more.
     max_seq_len: host-known upper bound of a sequence's keys; sizes the split of calls with few queries over many keys
-    (default: twice the mean of the sequences' rows).  sinks [Hq] / sliding_window as in `decode`, the window counted back from each query.
+    (default: Nk where that is at least three times Nq, else twice the mean of the sequences' keys).  sinks [Hq] /
+    sliding_window as in `decode`, the window counted back from each query.
     """
     lib = _lib.load()
     qs, ks, vs = _token_rows("q", q), _token_rows("k", k), _token_rows("v", v)

@@ -80,3 +80,11 @@ def test_a_window_past_32_bits_is_no_short_one():
         paged_attn._check_variant(None, -5, 4, None)
     assert paged_attn.packed_prefill_workspace_bytes(4, 400, 12600, 32, 8, 128, 3200, 2 ** 32 + 5) == \
         paged_attn.packed_prefill_workspace_bytes(4, 400, 12600, 32, 8, 128, 3200)
+
+
+def test_one_long_context_among_empty_ones_is_split_without_a_bound(lib):
+    """256 queries behind 32 K keys, alone and as one sequence of 64 whose others are empty: the mean says nothing there."""
+    for Hq, Hkv, D in ((32, 8, 128), (8, 2, 64)):
+        alone = _shares(lib, 1, 256, 33024, Hq, Hkv, D, 0)
+        assert alone == _shares(lib, 1, 256, 33024, Hq, Hkv, D, 33024) >= 8
+        assert _shares(lib, 64, 256, 33024, Hq, Hkv, D, 0) == _shares(lib, 64, 256, 33024, Hq, Hkv, D, 33024) >= 2
