@@ -243,7 +243,9 @@ void prefill_async_kernel(PrefillParams p) {
   // fused multiply-add per score, the accumulators starting at zero.  (With the
   // scale in Q, which rounds every element of it once more, the results of 32 prompts of 17-256 tokens are off by 1.5
   // times, of 4 096 cached keys by 2.2 times what their own rounding to bf16 costs, root mean square against float64;
-  // this way by 1.4 times, the rounding of the probabilities being the other part.  It costs 4 % on long prompts: 2 of 4 097-8 192 tokens, 869 -> 905 us.)
+  // this way by 1.4 times, the rounding of the probabilities being the other part.  It costs 4 % on long prompts: 2 of 4 097-8 192
+  // tokens, 869 -> 905 us.  The probabilities stay one bf16 operand: a second one for what they lose, as decode over int8
+  // pools has it, would be half as many matrix instructions again where these are what bounds a long prompt.)
   constexpr bool EXACT_Q = PACKED;
   constexpr int KS = DH / 16;                // k-steps of the score product
   constexpr int VC = DH / 32;                // 32-wide d chunks of the output
