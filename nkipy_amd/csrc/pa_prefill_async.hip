@@ -1095,7 +1095,7 @@ void prefill_async_kernel(PrefillParams p) {
         auto of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, r); };
         const int last = of(qlim), first = win > 0 ? max(last - win + 1, 0) : 0;      // the keys it sees
         const float l = __int_as_float(of(__float_as_int(l_run[j]))), m = __int_as_float(of(__float_as_int(m_ref[j])));
-        if (!(l < INFINITY)) continue;           // its scores are no numbers
+        if (l != l) continue;                    // its scores are no numbers (an infinite l is a sink's that leaves the keys nothing)
         uint32_t seen = 0, hidden = 0;           // of this lane's eight columns, those with a value that is no number
         auto scan = [&](int from, int to) __attribute__((always_inline)) {
 #pragma unroll 1

@@ -94,3 +94,13 @@ def test_a_chunk_over_an_int8_cache(pa):  # noqa: F811
     assert bool(torch.isfinite(got[0, :at]).all()) and torch.isfinite(got[1]).all()
     assert (got[0, :at].float() - want[0].float()).abs().max() <= 4 * 2.0 ** -8 * xv[0, :at].float().abs().max()
     assert bool(torch.isnan(got[0, at:, :4]).all()) and bool(torch.isnan(got[0, at:, 4:]).all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_sinks_that_leave_the_keys_nothing(pa, rng, D):  # noqa: F811
+    """A sink whose share of the sum is past float32's range: zeros, also for a row whose tile hides a NaN from it."""
+    Hq, Hkv, n = 4, 2, 100
+    q, k, v = (bf16(rng.standard_normal((n, h, D))) for h in (Hq, Hkv, Hkv))
+    v[70] = float("nan")
+    got = pa.packed_prefill(q, k, v, dev(_starts([n])), 0.1, sinks=torch.full((Hq,), 300.0, device="cuda"))
+    assert bool((got[:70] == 0).all()) and bool(torch.isnan(got[70:]).all())
