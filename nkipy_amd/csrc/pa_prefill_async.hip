@@ -1563,7 +1563,7 @@ int prefill_packed_splits(const PrefillParams& p, int num_cus) {
   // shares are shares of these keys.  32 / 8 heads of 128, 4 x 100 behind 3 K, us unsplit / in the five shares that its 3 200
   // keys without a window give: window 50 9.6 / 21.8, 128 12.2 / 26.9, 500 18.6 / 32.4; window 2 000, four shares, 49.7 / 36.2.
   long reach = bound;
-  if (p.window > 0) reach = std::min<long>(reach, p.window + (p.D == HD ? 128 / mult + 1 : 64) + 63);
+  if (p.window > 0) reach = std::min<long>(reach, (long)p.window + (p.D == HD ? 128 / mult + 1 : 64) + 63);
   // Head dim 64 with two q heads per wave: unsplit, a call of few workgroups runs with one (packed_form), twice as many of them,
   // so that the two-thirds are counted on those, and two shares are as many workgroups as none and always behind (us,
   // unsplit / 2 / 3 / 4 shares: 8 / 2 heads, 8 x 64 behind 1 000 21.1 / 26.3 / 22.7 / 21.5, 4 x 150 behind 2 K 36.1 / 40.9 / 33.0 /

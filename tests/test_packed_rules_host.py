@@ -88,3 +88,9 @@ def test_one_long_context_among_empty_ones_is_split_without_a_bound(lib):
         alone = _shares(lib, 1, 256, 33024, Hq, Hkv, D, 0)
         assert alone == _shares(lib, 1, 256, 33024, Hq, Hkv, D, 33024) >= 8
         assert _shares(lib, 64, 256, 33024, Hq, Hkv, D, 0) == _shares(lib, 64, 256, 33024, Hq, Hkv, D, 33024) >= 2
+
+
+def test_shares_under_the_longest_window_that_is_one(lib):
+    """A window a little shorter than 2^31 keys reaches as far as they do: the sum that says so is not of 32 bits."""
+    k = (1 << 31) - 1000
+    assert _shares(lib, 1, 64, k, 32, 8, 128, k, k - 1) == _shares(lib, 1, 64, k, 32, 8, 128, k) == 16
